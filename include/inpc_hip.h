@@ -563,6 +563,75 @@ int inpc_cauchy_loss(const float* input, const float* target, float* elementwise
 int inpc_cauchy_loss_backward(const float* grad, const float* input, const float* target,
                               float* grad_input, uint32_t n, void* stream);
 
+/* =========================================================================================
+ * Layers of the networks on either side of the rasterizer. The reference builds its own from torch's
+ * (Modules/UNet.py:1-200, the network behind the image; Modules/AppearanceField.py:1-88, the one in front): these
+ * calls have no counterpart among its kernels.
+ * ======================================================================================= */
+
+/* ---- element types and activations of the layers ------------------------------------------- */
+#define INPC_DTYPE_F32 0
+#define INPC_DTYPE_F16 1
+#define INPC_DTYPE_BF16 2
+#define INPC_ACTIVATION_NONE 0
+#define INPC_ACTIVATION_RELU 1 /* max(z, 0); slope 0 at 0                                   */
+#define INPC_ACTIVATION_SILU 2 /* z / (1 + exp(-z))                                         */
+#define INPC_ACTIVATION_GELU 3 /* z (1 + erf(z / sqrt 2)) / 2                               */
+
+/* Group norm over channels-last feature maps: n_images images of n_pixels pixels of `channels` adjacent
+ * values, the channels split into `groups` equal groups. Strides are in elements: from image to image and
+ * from pixel to pixel of the input (a slice of the channels of a wider map is an input like any other) and
+ * of the output's gradient (backward only); output and input gradient are dense. */
+#define INPC_GROUP_NORM_MAX_CHANNELS 65536u
+typedef struct inpc_group_norm_config {
+    uint32_t n_images, n_pixels; /* fewer than 2^30 pixels per image                              */
+    uint32_t channels, groups;
+    int32_t dtype;               /* of input, output and their gradients: INPC_DTYPE_*            */
+    int32_t param_dtype;         /* of weight, bias and their gradients: fp32 or `dtype`          */
+    int32_t activation;          /* INPC_ACTIVATION_*                                             */
+    float eps;
+    uint64_t input_image_stride, input_pixel_stride;
+    uint64_t grad_image_stride, grad_pixel_stride;
+    double dropout_p;            /* 0: no dropout. The rest as for inpc_dropout                   */
+    uint64_t seed;
+    const uint64_t* seed_dev;
+    uint64_t offset;
+} inpc_group_norm_config;
+
+/* The operators of the image network's blocks (Modules/UNet.py:1-200 takes its layers from torch):
+ *   xhat = (x - mean) / sqrt(var + eps), mean and biased variance over the pixels of an image and the channels
+ *   of a group; z = xhat * weight[c] + bias[c]; y = activation(z); with dropout_p > 0 then dropout of y, its
+ *   elements numbered ((image * n_pixels) + pixel) * channels + c.
+ * Computed in fp32 whatever the types; the output is rounded once. input, output: n_images * n_pixels *
+ * channels values; weight, bias (channels,) or NULL (1 and 0); moments (n_images * groups, 2) f32 dev receives
+ * {mean, 1 / sqrt(var + eps)} for the backward pass. Sums are added in an order that depends on the sizes
+ * and alignments alone: equal calls give equal bits. The workspace needs no clearing and holds nothing between calls.
+ * inpc_group_norm_workspace_bytes is 0 for a configuration that the calls refuse (inpc_last_error says why) and for
+ * an empty one. No host synchronisation, no memory but the caller's: all calls can be captured into a graph. */
+size_t inpc_group_norm_workspace_bytes(const inpc_group_norm_config* cfg);
+int inpc_group_norm_forward(const inpc_group_norm_config* cfg, const void* input, const void* weight,
+                            const void* bias, void* output, float* moments, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Gradients of the same (the layers of Modules/UNet.py:1-200): grad_input dense like the output, grad_weight and
+ * grad_bias (channels,) of param_dtype; any of the three may be NULL. `moments` is what the forward call wrote;
+ * seed (or what seed_dev points to) and offset have to be those of the forward call: the mask is
+ * computed again. */
+int inpc_group_norm_backward(const inpc_group_norm_config* cfg, const void* grad_output,
+                             const void* input, const void* weight, const void* bias,
+                             const float* moments, void* grad_input, void* grad_weight,
+                             void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* output[i] = 0 where u(i) < round(p * 2^32), else input[i] / (1 - p), computed in fp32 and rounded once (dropout of
+ * hidden features, which a network like Modules/AppearanceField.py:1-88 takes from torch). The mask is stored nowhere:
+ * u(i) = h(0, i) * 2^16 + h(1, i), and h(d, i) is the 16-bit half i mod 8, low halves first, of the four words of
+ * Philox4x32-10 with the seed as its key (low word first) and the counter (b mod 2^32, b div 2^32 + 2^31 d,
+ * offset mod 2^32, offset div 2^32), b = i div 8. The backward pass is the same call on the gradient.
+ * seed_dev, where not NULL, is read on the device in place of `seed`: a captured call then draws a new mask on
+ * every replay whose seed was changed. output may be input. count < 2^40; p = 1 drops everything. */
+int inpc_dropout(const void* input, void* output, uint64_t count, int dtype, double p,
+                 uint64_t seed, const uint64_t* seed_dev, uint64_t offset, void* stream);
+
 /* Per-kernel timing hooks for benchmarks: when enabled, every launch made by the calling
  * thread is bracketed by HIP events on its stream; inpc_timing_collect synchronises and
  * returns the number of records written as {name, milliseconds}. */

@@ -20,6 +20,8 @@ FEAT_RAW37_F16 = 3
 RASTER_INFERENCE = 1
 RASTER_KEEP_GEOMETRY = 2
 CULL_IF_COMPLETE = 0xFFFFFFFF  # INPC_CULL_IF_COMPLETE
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+ACTIVATION_NONE, ACTIVATION_RELU, ACTIVATION_SILU, ACTIVATION_GELU = 0, 1, 2, 3
 CDF_HEAD_MIN_FLOATS = 16384  # INPC_CDF_HEAD_MIN_FLOATS: the smallest CDF head; inpc_cdf_head_floats(n_leaves) sizes one
 
 
@@ -99,6 +101,27 @@ class GaussianLayout(C.Structure):
     ]
 
 
+class GroupNormConfig(C.Structure):
+    _fields_ = [
+        ("n_images", C.c_uint32),
+        ("n_pixels", C.c_uint32),
+        ("channels", C.c_uint32),
+        ("groups", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("param_dtype", C.c_int32),
+        ("activation", C.c_int32),
+        ("eps", C.c_float),
+        ("input_image_stride", C.c_uint64),
+        ("input_pixel_stride", C.c_uint64),
+        ("grad_image_stride", C.c_uint64),
+        ("grad_pixel_stride", C.c_uint64),
+        ("dropout_p", C.c_double),
+        ("seed", C.c_uint64),
+        ("seed_dev", C.c_void_p),
+        ("offset", C.c_uint64),
+    ]
+
+
 class TimingRecord(C.Structure):
     _fields_ = [("name", C.c_char_p), ("ms", C.c_float)]
 
@@ -111,6 +134,7 @@ _SZ = C.c_size_t
 _CAM = C.POINTER(Camera)
 _CFG = C.POINTER(RasterConfig)
 _GCFG = C.POINTER(GaussianConfig)
+_NCFG = C.POINTER(GroupNormConfig)
 SIGNATURES = {
     "inpc_last_error": (C.c_char_p, []),
     "inpc_abi_version": (C.c_int, []),
@@ -161,6 +185,10 @@ SIGNATURES = {
     "inpc_weight_decay_grads": (C.c_int, [_P, _P, _U32, C.c_int, _P]),
     "inpc_cauchy_loss": (C.c_int, [_P, _P, _P, _U32, _P]),
     "inpc_cauchy_loss_backward": (C.c_int, [_P, _P, _P, _P, _U32, _P]),
+    "inpc_group_norm_workspace_bytes": (_SZ, [_NCFG]),
+    "inpc_group_norm_forward": (C.c_int, [_NCFG, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "inpc_group_norm_backward": (C.c_int, [_NCFG, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "inpc_dropout": (C.c_int, [_P, _P, C.c_uint64, C.c_int, C.c_double, C.c_uint64, _P, C.c_uint64, _P]),
     "inpc_timing_enable": (None, [C.c_int]),
     "inpc_timing_collect": (C.c_int, [C.POINTER(TimingRecord), C.c_int]),
     "inpc_calibration_copy": (C.c_int, [_P, _P, _SZ, _P]),

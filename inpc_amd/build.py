@@ -15,7 +15,8 @@ CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libinpc_hip.so"
 RESOURCES_PATH = PKG_DIR / "kernel_resources.json"   # what the compiler reports per kernel, written with the library
 SOURCES = ["runtime.hip", "sampler.hip", "raster.hip", "field.hip", "misc.hip"]
-HEADERS = ["common.hpp", "geometry.hpp", "blend.hpp", "tilesort.hpp", "gaussian.hpp"]
+HEADERS = ["common.hpp", "geometry.hpp", "blend.hpp", "tilesort.hpp", "gaussian.hpp", "elements.hpp", "groupnorm.hpp",
+           "dropout.hpp"]
 
 # -ffp-contract=off: tile bounds, depth keys, leaf picks and cull decisions must be bit-identical to
 #   a CPU evaluation of the same expressions, so nothing may be fused behind the source's back.

@@ -1,0 +1,59 @@
+// dropout.hpp — y = 0 where the mask drops the element, x / (1 - p) elsewhere; the backward pass is the same map on the
+// gradient, with the mask computed again (elements.hpp) instead of stored.
+#pragma once
+
+#include "elements.hpp"
+
+namespace inpc {
+namespace dropout {
+
+constexpr int kBlock = 256;
+
+// A thread takes eight consecutive elements, one draw of the generator. WIDE: both pointers are 16-byte aligned.
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(kBlock) k_dropout(const void* __restrict__ x, void* __restrict__ y, uint64_t count, Dropout d) {
+    const uint64_t first = ((uint64_t)blockIdx.x * kBlock + threadIdx.x) * 8u;
+    if (first >= count) return;
+    const uint64_t seed = dropout_seed(d);
+    constexpr int W = D == INPC_DTYPE_F32 ? 4 : 8;
+    float v[8];
+    if (WIDE && first + 8 <= count) {
+        float part[W];
+#pragma unroll
+        for (int k = 0; k < 8 / W; ++k) {
+            load_vector<D, W>(x, first + k * W, part);
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[k * W + j] = part[j];
+        }
+        dropout_apply<8>(d, seed, first, v);
+#pragma unroll
+        for (int k = 0; k < 8 / W; ++k) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) part[j] = v[k * W + j];
+            store_vector<D, W>(y, first + k * W, part);
+        }
+        return;
+    }
+    const uint32_t kept = dropout_kept<8>(d, seed, first);
+    const uint32_t n = (uint32_t)min((unsigned long long)(count - first), 8ull);
+    for (uint32_t j = 0; j < n; ++j) {
+        float one[1];
+        load_vector<D, 1>(x, first + j, one);
+        one[0] = (kept >> j) & 1u ? rounded_product(one[0], d.scale) : 0.0f;
+        store_vector<D, 1>(y, first + j, one);
+    }
+}
+
+template <int D>
+int launch(const void* x, void* y, uint64_t count, const Dropout& d, hipStream_t stream) {
+    const uint32_t blocks = (uint32_t)((count + 8 * kBlock - 1) / (8 * kBlock));
+    if (((uintptr_t)x | (uintptr_t)y) % 16 == 0) {
+        INPC_LAUNCH("dropout", (k_dropout<D, true>), dim3(blocks), dim3(kBlock), stream, x, y, count, d);
+    } else {
+        INPC_LAUNCH("dropout", (k_dropout<D, false>), dim3(blocks), dim3(kBlock), stream, x, y, count, d);
+    }
+    return INPC_OK;
+}
+
+}  // namespace dropout
+}  // namespace inpc

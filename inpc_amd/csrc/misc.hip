@@ -2,9 +2,13 @@
 // the rasterizer's input:
 //   spherical contraction of the sample positions   (B/misc/src/misc_kernels.cu:49-66)
 //   raw density feature -> opacity and its gradient  (feature_to_opacity / TruncExp, utils.py:13-33)
+// and the layers of the networks there that the reference leaves to torch: group norm with an activation (groupnorm.hpp) and
+// dropout (dropout.hpp).
 #include <algorithm>
 
 #include "common.hpp"
+#include "dropout.hpp"
+#include "groupnorm.hpp"
 
 namespace inpc {
 namespace {
@@ -162,6 +166,59 @@ int inpc_cauchy_loss_backward(const float* grad, const float* input, const float
     INPC_LAUNCH("cauchy_loss_backward", k_cauchy_loss_backward, dim3(grid_for(n)), dim3(kBlock), (hipStream_t)stream, grad,
                 input, target, grad_input, n);
     return INPC_OK;
+}
+
+size_t inpc_group_norm_workspace_bytes(const inpc_group_norm_config* cfg) {
+    using namespace inpc;
+    if (norm::check_config(cfg, "group_norm_workspace_bytes") != INPC_OK) return 0;
+    if (cfg->n_images == 0 || cfg->n_pixels == 0) return 0;
+    return norm::workspace_of(*cfg).bytes;
+}
+
+int inpc_group_norm_forward(const inpc_group_norm_config* cfg, const void* input, const void* weight, const void* bias,
+                            void* output, float* moments, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace inpc;
+    if (const int rc = norm::check_config(cfg, "group_norm_forward")) return rc;
+    if (cfg->n_images == 0 || cfg->n_pixels == 0) return INPC_OK;
+    if (!input || !output || !moments) return fail(INPC_E_INVALID_ARGUMENT, "group_norm_forward: null pointer");
+    if (const int rc = norm::check_workspace(*cfg, workspace, workspace_bytes, "group_norm_forward")) return rc;
+    const size_t bytes = element_bytes(cfg->dtype);
+    const int v = norm::vector_width(bytes, cfg->channels | cfg->input_image_stride | cfg->input_pixel_stride,
+                                     (uintptr_t)input | (uintptr_t)output);
+    return INPC_NORM_DISPATCH(norm::forward, cfg->dtype, v, *cfg, input, weight, bias, output, (float2*)moments, (char*)workspace,
+                              (hipStream_t)stream);
+}
+
+int inpc_group_norm_backward(const inpc_group_norm_config* cfg, const void* grad_output, const void* input, const void* weight,
+                             const void* bias, const float* moments, void* grad_input, void* grad_weight, void* grad_bias,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace inpc;
+    if (const int rc = norm::check_config(cfg, "group_norm_backward")) return rc;
+    if (cfg->n_images == 0 || cfg->n_pixels == 0 || !(grad_input || grad_weight || grad_bias)) return INPC_OK;
+    if (!grad_output || !input || !moments) return fail(INPC_E_INVALID_ARGUMENT, "group_norm_backward: null pointer");
+    if (const int rc = norm::check_workspace(*cfg, workspace, workspace_bytes, "group_norm_backward")) return rc;
+    const size_t bytes = element_bytes(cfg->dtype);
+    const int v = norm::vector_width(bytes, cfg->channels | cfg->input_image_stride | cfg->input_pixel_stride |
+                                                cfg->grad_image_stride | cfg->grad_pixel_stride,
+                                     (uintptr_t)input | (uintptr_t)grad_output | (uintptr_t)grad_input);
+    return INPC_NORM_DISPATCH(norm::backward, cfg->dtype, v, *cfg, input, grad_output, (const float2*)moments, weight, bias,
+                              grad_input, grad_weight, grad_bias, (char*)workspace, (hipStream_t)stream);
+}
+
+int inpc_dropout(const void* input, void* output, uint64_t count, int dtype, double p, uint64_t seed, const uint64_t* seed_dev,
+                 uint64_t offset, void* stream) {
+    using namespace inpc;
+    if (!known_dtype(dtype)) return fail(INPC_E_UNSUPPORTED, "dropout: values are fp32, fp16 or bf16");
+    if (!valid_probability(p)) return fail(INPC_E_INVALID_ARGUMENT, "dropout: the probability is outside [0, 1]");
+    if (count == 0) return INPC_OK;
+    if (!input || !output) return fail(INPC_E_INVALID_ARGUMENT, "dropout: null pointer");
+    if (count >= (1ull << 40)) return fail(INPC_E_UNSUPPORTED, "dropout: fewer than 2^40 values per call");
+    const Dropout d = make_dropout(p, seed, seed_dev, offset);
+    switch (dtype) {
+        case INPC_DTYPE_F32: return dropout::launch<INPC_DTYPE_F32>(input, output, count, d, (hipStream_t)stream);
+        case INPC_DTYPE_F16: return dropout::launch<INPC_DTYPE_F16>(input, output, count, d, (hipStream_t)stream);
+        default: return dropout::launch<INPC_DTYPE_BF16>(input, output, count, d, (hipStream_t)stream);
+    }
 }
 
 }  // extern "C"

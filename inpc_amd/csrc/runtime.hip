@@ -204,7 +204,7 @@ int inpc_calibration_copy(const void* src, void* dst, size_t bytes, void* stream
 
 const char* inpc_last_error(void) { return inpc::g_error; }
 
-int inpc_abi_version(void) { return 4; }
+int inpc_abi_version(void) { return 5; }
 
 int inpc_side_stream_policy(int existing, int stream_is_capturing, int second_is_capturing, int n_kept) {
     return (int)inpc::choose_lane(existing != 0, stream_is_capturing != 0, second_is_capturing != 0, n_kept);

@@ -1,0 +1,228 @@
+"""Layers of the networks on either side of the rasterizer: group norm with an activation over channels-last feature
+maps (with dropout behind it if asked for), and dropout from a counter-based generator. The reference builds its
+networks from torch's layers (Modules/UNet.py:1-200, Modules/AppearanceField.py:1-88); these two compute in fp32, run as
+hand-written kernels in both directions and keep neither normalised values nor masks for the backward pass.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from typing import Any
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+_ACTIVATIONS = {"none": _lib.ACTIVATION_NONE, "relu": _lib.ACTIVATION_RELU, "silu": _lib.ACTIVATION_SILU,
+                "gelu": _lib.ACTIVATION_GELU}
+
+
+def _on_device_of(t: torch.Tensor):
+    """The library launches on the current device: make it the tensor's."""
+    if t.device.type == "cuda" and t.device.index != torch.cuda.current_device():
+        return torch.cuda.device(t.device)
+    return contextlib.nullcontext()
+
+
+def _require_values(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"expected {name} to be a tensor on the GPU")
+    if t.dtype not in _DTYPES:
+        raise RuntimeError(f"expected {name} of scalar type Float, Half or BFloat16, got {t.dtype}")
+
+
+def _require_probability(p: float, name: str) -> float:
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{name} must lie in [0, 1], got {p}")
+    return p
+
+
+def _require_seed(seed: int | torch.Tensor | None, offset: int, device: torch.device) -> tuple[int, torch.Tensor | None, int]:
+    """(seed, its place on the GPU or None, offset)"""
+    if isinstance(offset, bool) or not isinstance(offset, int) or not 0 <= offset < 2**64:
+        raise ValueError("offset must be a whole number in [0, 2^64)")
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
+            raise RuntimeError("a seed tensor holds one Long on the device of the input")
+        return 0, seed, offset
+    if seed is None or isinstance(seed, bool) or not isinstance(seed, int) or not 0 <= seed < 2**64:
+        raise ValueError("dropout needs a seed: a whole number in [0, 2^64) or a tensor that holds one")
+    return seed, None, offset
+
+
+# ---- dropout -------------------------------------------------------------------------------------------------------
+
+def _memory_format(t: torch.Tensor) -> torch.memory_format:
+    """The order in which a tensor's elements are numbered: channels last where that is how it lies in memory."""
+    if t.dim() == 4 and not t.is_contiguous() and t.is_contiguous(memory_format=torch.channels_last):
+        return torch.channels_last
+    return torch.contiguous_format
+
+
+def _dropout_call(x: torch.Tensor, p: float, seed: int, seed_tensor: torch.Tensor | None, offset: int) -> torch.Tensor:
+    out = torch.empty_like(x)
+    with _on_device_of(x):
+        _lib.check(_lib.lib().inpc_dropout(_lib.ptr(x), _lib.ptr(out), x.numel(), _DTYPES[x.dtype], p, seed,
+                                           _lib.ptr(seed_tensor), offset, _lib.current_stream()), "inpc_dropout")
+    return out
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x: torch.Tensor, p: float, seed: int, seed_tensor: torch.Tensor | None, offset: int) -> torch.Tensor:
+        order = _memory_format(x)
+        ctx.args = p, seed, offset, order
+        ctx.save_for_backward(seed_tensor)
+        return _dropout_call(x.contiguous(memory_format=order), p, seed, seed_tensor, offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad: torch.Tensor):
+        p, seed, offset, order = ctx.args
+        (seed_tensor,) = ctx.saved_tensors
+        return _dropout_call(grad.contiguous(memory_format=order), p, seed, seed_tensor, offset), None, None, None, None
+
+
+def dropout(input: torch.Tensor, p: float, seed: int | torch.Tensor | None, offset: int = 0, training: bool = True) -> torch.Tensor:
+    """Zeroes each element of `input` with probability `p` and divides the others by 1 - p; differentiable.
+
+    The mask is a function of `seed`, `offset` and an element's number in memory order alone (channels-last tensors
+    are numbered that way, all others row-major; tensors that are neither are made contiguous first) and is stored nowhere: the
+    backward pass computes it again. Calls with different `seed` or `offset` draw independent masks, so use one seed for
+    a training run and step the offset from layer to layer, and another seed for each iteration. `seed` is a whole
+    number or a GPU tensor of one int64, which is read when the kernel runs (in a captured graph: on every
+    replay); torch refuses a backward pass if that tensor has been changed in between. The generator is
+    Philox4x32-10; include/inpc_hip.h (inpc_dropout) gives the numbering of its bits. With training=False or p = 0,
+    `input` itself is returned.
+    """
+    _require_values(input, "input")
+    p = _require_probability(p, "p")
+    if not training or p == 0.0:
+        return input
+    return _Dropout.apply(input, p, *_require_seed(seed, offset, input.device))
+
+
+# ---- group norm ----------------------------------------------------------------------------------------------------
+
+def _pixel_strides(t: torch.Tensor) -> tuple[int, int] | None:
+    """(from image to image, from pixel to pixel) of a (N, C, H, W) tensor whose channels are adjacent and whose pixels lie
+    evenly spaced; None where it lies otherwise. Strides of dimensions of size one mean nothing."""
+    n, c, h, w = t.shape
+    s_n, s_c, s_h, s_w = t.stride()
+    if c != 1 and s_c != 1:
+        return None
+    if w != 1:
+        pixel = s_w
+        if h != 1 and s_h != w * s_w:
+            return None
+    else:
+        pixel = s_h if h != 1 else c
+    image = s_n if n != 1 else h * w * pixel
+    if pixel < c or image < h * w * pixel:   # overlapping or expanded
+        return None
+    return image, pixel
+
+
+def _channels_last(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """The tensor, copied to a dense channels-last one where the kernels cannot read it as it lies, and its strides."""
+    strides = _pixel_strides(t)
+    if strides is None:
+        n, c, h, w = t.shape
+        out = _dense(t)
+        out.copy_(t)
+        return out, h * w * c, c
+    return t, *strides
+
+
+def _dense(like: torch.Tensor) -> torch.Tensor:
+    """An uninitialised (N, C, H, W) tensor that lies as (N, H, W, C)."""
+    n, c, h, w = like.shape
+    return torch.empty((n, h, w, c), dtype=like.dtype, device=like.device).permute(0, 3, 1, 2)
+
+
+def _workspace(cfg: _lib.GroupNormConfig, device: torch.device) -> tuple[torch.Tensor | None, int]:
+    size = _lib.lib().inpc_group_norm_workspace_bytes(C.byref(cfg))
+    return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, groups: int, eps: float,
+                activation: int, p: float, seed: int, seed_tensor: torch.Tensor | None, offset: int) -> torch.Tensor:
+        x, image_stride, pixel_stride = _channels_last(x)
+        n, c, h, w = x.shape
+        param_dtype = next((_DTYPES[t.dtype] for t in (weight, bias) if t is not None), _lib.DTYPE_F32)
+        cfg = _lib.GroupNormConfig(n, h * w, c, groups, _DTYPES[x.dtype], param_dtype, activation, eps, image_stride,
+                                   pixel_stride, 0, 0, p, seed, None if seed_tensor is None else seed_tensor.data_ptr(), offset)
+        y = _dense(x)
+        moments = torch.empty((n * groups, 2), dtype=torch.float32, device=x.device)
+        with _on_device_of(x):
+            workspace, size = _workspace(cfg, x.device)
+            _lib.check(_lib.lib().inpc_group_norm_forward(C.byref(cfg), _lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias),
+                                                          _lib.ptr(y), _lib.ptr(moments), _lib.ptr(workspace), size,
+                                                          _lib.current_stream()), "inpc_group_norm_forward")
+        ctx.cfg = cfg
+        ctx.save_for_backward(x, weight, bias, moments, seed_tensor)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad: torch.Tensor):
+        x, weight, bias, moments, seed_tensor = ctx.saved_tensors
+        cfg = _lib.GroupNormConfig.from_buffer_copy(ctx.cfg)
+        grad, cfg.grad_image_stride, cfg.grad_pixel_stride = _channels_last(grad)
+        need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
+        zeros = torch.zeros_like if x.numel() == 0 else torch.empty_like
+        dx = _dense(x) if need_x else None
+        dweight = zeros(weight, memory_format=torch.contiguous_format) if need_weight else None
+        dbias = zeros(bias, memory_format=torch.contiguous_format) if need_bias else None
+        with _on_device_of(x):
+            workspace, size = _workspace(cfg, x.device)
+            _lib.check(_lib.lib().inpc_group_norm_backward(C.byref(cfg), _lib.ptr(grad), _lib.ptr(x), _lib.ptr(weight),
+                                                           _lib.ptr(bias), _lib.ptr(moments), _lib.ptr(dx), _lib.ptr(dweight),
+                                                           _lib.ptr(dbias), _lib.ptr(workspace), size, _lib.current_stream()),
+                       "inpc_group_norm_backward")
+        return dx, dweight, dbias, None, None, None, None, None, None, None
+
+
+def group_norm(input: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, activation: str = "none", dropout_p: float = 0.0, seed: int | torch.Tensor | None = None,
+               offset: int = 0, training: bool = True) -> torch.Tensor:
+    """Group norm of a (N, C, H, W) feature map, then an activation ("none", "relu", "silu" or "gelu", the exact one), then
+    dropout where dropout_p > 0; differentiable in `input`, `weight` and `bias`.
+
+    The kernels work on channels-last maps (torch.channels_last, also a slice of the channels of a wider one); other
+    layouts are copied into that first. The result is a dense channels-last tensor of the input's type. `weight`
+    and `bias` are (C,) tensors of one type, fp32 or the input's, so fp32 parameters serve 16-bit maps. Everything is computed in fp32 and rounded
+    once, at the end of the whole chain. `dropout_p`, `seed`, `offset` and `training` are those of `dropout`, which
+    gives the same mask for the same map. For the backward pass only the input and two numbers per image
+    and group are kept.
+    """
+    _require_values(input, "input")
+    if input.dim() != 4:
+        raise ValueError(f"expected a (N, C, H, W) tensor, got {input.dim()} dimensions")
+    channels = input.shape[1]
+    if input.shape[2] * input.shape[3] >= 2**30 or input.shape[0] >= 2**31:
+        raise ValueError("expected fewer than 2^30 pixels per image and fewer than 2^31 images")
+    if isinstance(num_groups, bool) or not isinstance(num_groups, int) or num_groups < 1 or channels < 1 or channels % num_groups != 0:
+        raise ValueError(f"{channels} channels cannot be split into {num_groups} groups")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}; choose from {', '.join(_ACTIVATIONS)}")
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.shape != (channels,):
+            raise ValueError(f"expected {name} of shape ({channels},), got {tuple(t.shape)}")
+        if t.dtype not in (torch.float32, input.dtype) or (weight is not None and bias is not None and weight.dtype != bias.dtype):
+            raise RuntimeError("weight and bias have one scalar type, Float or that of the input")
+        if t.device != input.device:
+            raise RuntimeError("expected all tensors on the same device")
+    p = _require_probability(dropout_p, "dropout_p") if training else 0.0
+    seed, seed_tensor, offset = _require_seed(seed, offset, input.device) if p > 0.0 else (0, None, 0)
+    weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
+    return _GroupNorm.apply(input, weight, bias, num_groups, float(eps), _ACTIVATIONS[activation], p, seed, seed_tensor, offset)
