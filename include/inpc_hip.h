@@ -606,9 +606,9 @@ typedef struct inpc_group_norm_config {
  * channels values; weight, bias (channels,) or NULL (1 and 0); moments (n_images * groups, 2) f32 dev receives
  * {mean, 1 / sqrt(var + eps)} for the backward pass. Sums are added in an order that depends on the sizes
  * and alignments alone: equal calls give equal bits. The workspace needs no clearing and holds nothing between calls.
- * inpc_group_norm_workspace_bytes is 0 for a configuration that the calls refuse (inpc_last_error says why) and for
- * an empty one. No host synchronisation, no memory but the caller's: all calls can be captured into a graph. */
-size_t inpc_group_norm_workspace_bytes(const inpc_group_norm_config* cfg);
+ * inpc_group_norm_workspace_bytes (backward = 0: of the forward call, 1: of the backward call) is 0 where none is
+ * needed and for a configuration that the calls refuse (inpc_last_error says why). No host synchronisation, no memory but the caller's: all calls can be captured into a graph. */
+size_t inpc_group_norm_workspace_bytes(const inpc_group_norm_config* cfg, int backward);
 int inpc_group_norm_forward(const inpc_group_norm_config* cfg, const void* input, const void* weight,
                             const void* bias, void* output, float* moments, void* workspace,
                             size_t workspace_bytes, void* stream);

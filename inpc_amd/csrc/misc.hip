@@ -168,11 +168,11 @@ int inpc_cauchy_loss_backward(const float* grad, const float* input, const float
     return INPC_OK;
 }
 
-size_t inpc_group_norm_workspace_bytes(const inpc_group_norm_config* cfg) {
+size_t inpc_group_norm_workspace_bytes(const inpc_group_norm_config* cfg, int backward) {
     using namespace inpc;
     if (norm::check_config(cfg, "group_norm_workspace_bytes") != INPC_OK) return 0;
     if (cfg->n_images == 0 || cfg->n_pixels == 0) return 0;
-    return norm::workspace_of(*cfg).bytes;
+    return norm::workspace_bytes(*cfg, backward != 0);
 }
 
 int inpc_group_norm_forward(const inpc_group_norm_config* cfg, const void* input, const void* weight, const void* bias,
@@ -181,12 +181,8 @@ int inpc_group_norm_forward(const inpc_group_norm_config* cfg, const void* input
     if (const int rc = norm::check_config(cfg, "group_norm_forward")) return rc;
     if (cfg->n_images == 0 || cfg->n_pixels == 0) return INPC_OK;
     if (!input || !output || !moments) return fail(INPC_E_INVALID_ARGUMENT, "group_norm_forward: null pointer");
-    if (const int rc = norm::check_workspace(*cfg, workspace, workspace_bytes, "group_norm_forward")) return rc;
-    const size_t bytes = element_bytes(cfg->dtype);
-    const int v = norm::vector_width(bytes, cfg->channels | cfg->input_image_stride | cfg->input_pixel_stride,
-                                     (uintptr_t)input | (uintptr_t)output);
-    return INPC_NORM_DISPATCH(norm::forward, cfg->dtype, v, *cfg, input, weight, bias, output, (float2*)moments, (char*)workspace,
-                              (hipStream_t)stream);
+    if (const int rc = norm::check_workspace(*cfg, false, workspace, workspace_bytes, "group_norm_forward")) return rc;
+    return norm::forward(*cfg, input, weight, bias, output, (float2*)moments, (char*)workspace, (hipStream_t)stream);
 }
 
 int inpc_group_norm_backward(const inpc_group_norm_config* cfg, const void* grad_output, const void* input, const void* weight,
@@ -196,13 +192,9 @@ int inpc_group_norm_backward(const inpc_group_norm_config* cfg, const void* grad
     if (const int rc = norm::check_config(cfg, "group_norm_backward")) return rc;
     if (cfg->n_images == 0 || cfg->n_pixels == 0 || !(grad_input || grad_weight || grad_bias)) return INPC_OK;
     if (!grad_output || !input || !moments) return fail(INPC_E_INVALID_ARGUMENT, "group_norm_backward: null pointer");
-    if (const int rc = norm::check_workspace(*cfg, workspace, workspace_bytes, "group_norm_backward")) return rc;
-    const size_t bytes = element_bytes(cfg->dtype);
-    const int v = norm::vector_width(bytes, cfg->channels | cfg->input_image_stride | cfg->input_pixel_stride |
-                                                cfg->grad_image_stride | cfg->grad_pixel_stride,
-                                     (uintptr_t)input | (uintptr_t)grad_output | (uintptr_t)grad_input);
-    return INPC_NORM_DISPATCH(norm::backward, cfg->dtype, v, *cfg, input, grad_output, (const float2*)moments, weight, bias,
-                              grad_input, grad_weight, grad_bias, (char*)workspace, (hipStream_t)stream);
+    if (const int rc = norm::check_workspace(*cfg, true, workspace, workspace_bytes, "group_norm_backward")) return rc;
+    return norm::backward(*cfg, input, grad_output, (const float2*)moments, weight, bias, grad_input, grad_weight, grad_bias,
+                          (char*)workspace, (hipStream_t)stream);
 }
 
 int inpc_dropout(const void* input, void* output, uint64_t count, int dtype, double p, uint64_t seed, const uint64_t* seed_dev,

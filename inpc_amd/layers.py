@@ -5,7 +5,6 @@ hand-written kernels in both directions and keep neither normalised values nor m
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 from typing import Any
 
@@ -19,11 +18,19 @@ _ACTIVATIONS = {"none": _lib.ACTIVATION_NONE, "relu": _lib.ACTIVATION_RELU, "sil
                 "gelu": _lib.ACTIVATION_GELU}
 
 
-def _on_device_of(t: torch.Tensor):
-    """The library launches on the current device: make it the tensor's."""
-    if t.device.type == "cuda" and t.device.index != torch.cuda.current_device():
-        return torch.cuda.device(t.device)
-    return contextlib.nullcontext()
+def _run(name: str, t: torch.Tensor, *args) -> None:
+    """Calls the library with `args` and the current stream of the device that `t` lies on. The library launches on the
+    current device, so that is made the tensor's."""
+    index = t.get_device()
+    if index >= 0 and index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            _lib.check(getattr(_lib.lib(), name)(*args, _lib.current_stream()), name)
+    else:
+        _lib.check(getattr(_lib.lib(), name)(*args, _lib.current_stream()), name)
+
+
+def _address(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _require_values(t: torch.Tensor, name: str) -> None:
@@ -64,26 +71,23 @@ def _memory_format(t: torch.Tensor) -> torch.memory_format:
 
 def _dropout_call(x: torch.Tensor, p: float, seed: int, seed_tensor: torch.Tensor | None, offset: int) -> torch.Tensor:
     out = torch.empty_like(x)
-    with _on_device_of(x):
-        _lib.check(_lib.lib().inpc_dropout(_lib.ptr(x), _lib.ptr(out), x.numel(), _DTYPES[x.dtype], p, seed,
-                                           _lib.ptr(seed_tensor), offset, _lib.current_stream()), "inpc_dropout")
+    _run("inpc_dropout", x, x.data_ptr(), out.data_ptr(), x.numel(), _DTYPES[x.dtype], p, seed, _address(seed_tensor), offset)
     return out
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, x: torch.Tensor, p: float, seed: int, seed_tensor: torch.Tensor | None, offset: int) -> torch.Tensor:
-        order = _memory_format(x)
-        ctx.args = p, seed, offset, order
-        ctx.save_for_backward(seed_tensor)
-        return _dropout_call(x.contiguous(memory_format=order), p, seed, seed_tensor, offset)
+    def forward(ctx: Any, x: torch.Tensor, order: torch.memory_format, random: tuple) -> torch.Tensor:
+        ctx.order, ctx.random = order, random
+        if random[2] is not None:
+            ctx.save_for_backward(random[2])   # torch watches over it
+        return _dropout_call(x, *random)
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):
-        p, seed, offset, order = ctx.args
-        (seed_tensor,) = ctx.saved_tensors
-        return _dropout_call(grad.contiguous(memory_format=order), p, seed, seed_tensor, offset), None, None, None, None
+        ctx.saved_tensors
+        return _dropout_call(grad.contiguous(memory_format=ctx.order), *ctx.random), None, None
 
 
 def dropout(input: torch.Tensor, p: float, seed: int | torch.Tensor | None, offset: int = 0, training: bool = True) -> torch.Tensor:
@@ -102,7 +106,12 @@ def dropout(input: torch.Tensor, p: float, seed: int | torch.Tensor | None, offs
     p = _require_probability(p, "p")
     if not training or p == 0.0:
         return input
-    return _Dropout.apply(input, p, *_require_seed(seed, offset, input.device))
+    random = (p, *_require_seed(seed, offset, input.device))
+    order = _memory_format(input)
+    input = input.contiguous(memory_format=order)
+    if torch.is_grad_enabled() and input.requires_grad:
+        return _Dropout.apply(input, order, random)
+    return _dropout_call(input, *random)
 
 
 # ---- group norm ----------------------------------------------------------------------------------------------------
@@ -112,6 +121,8 @@ def _pixel_strides(t: torch.Tensor) -> tuple[int, int] | None:
     evenly spaced; None where it lies otherwise. Strides of dimensions of size one mean nothing."""
     n, c, h, w = t.shape
     s_n, s_c, s_h, s_w = t.stride()
+    if s_c == 1 and s_w == c and s_h == w * c and s_n == h * w * c:   # dense
+        return s_n, c
     if c != 1 and s_c != 1:
         return None
     if w != 1:
@@ -126,66 +137,64 @@ def _pixel_strides(t: torch.Tensor) -> tuple[int, int] | None:
     return image, pixel
 
 
+def _dense(like: torch.Tensor) -> torch.Tensor:
+    """An uninitialised (N, C, H, W) tensor that lies as (N, H, W, C)."""
+    n, c, h, w = like.shape
+    return torch.empty_strided((n, c, h, w), (h * w * c, 1, w * c, c), dtype=like.dtype, device=like.device)
+
+
 def _channels_last(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """The tensor, copied to a dense channels-last one where the kernels cannot read it as it lies, and its strides."""
     strides = _pixel_strides(t)
     if strides is None:
-        n, c, h, w = t.shape
-        out = _dense(t)
-        out.copy_(t)
-        return out, h * w * c, c
+        t = _dense(t).copy_(t)
+        strides = _pixel_strides(t)
     return t, *strides
 
 
-def _dense(like: torch.Tensor) -> torch.Tensor:
-    """An uninitialised (N, C, H, W) tensor that lies as (N, H, W, C)."""
-    n, c, h, w = like.shape
-    return torch.empty((n, h, w, c), dtype=like.dtype, device=like.device).permute(0, 3, 1, 2)
-
-
-def _workspace(cfg: _lib.GroupNormConfig, device: torch.device) -> tuple[torch.Tensor | None, int]:
-    size = _lib.lib().inpc_group_norm_workspace_bytes(C.byref(cfg))
+def _workspace(cfg: _lib.GroupNormConfig, backward: int, device: torch.device) -> tuple[torch.Tensor | None, int]:
+    size = _lib.lib().inpc_group_norm_workspace_bytes(C.byref(cfg), backward)
     return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+
+
+def _group_norm_call(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, groups: int, eps: float,
+                     activation: int, p: float, seed: int, seed_tensor: torch.Tensor | None, offset: int):
+    """(output, the input as the kernels have read it, moments, configuration)"""
+    x, image_stride, pixel_stride = _channels_last(x)
+    n, c, h, w = x.shape
+    param = weight if weight is not None else bias
+    cfg = _lib.GroupNormConfig(n, h * w, c, groups, _DTYPES[x.dtype], _lib.DTYPE_F32 if param is None else _DTYPES[param.dtype],
+                               activation, eps, image_stride, pixel_stride, 0, 0, p, seed, _address(seed_tensor), offset)
+    y = _dense(x)
+    moments = torch.empty(2 * n * groups, dtype=torch.float32, device=x.device)
+    workspace, size = _workspace(cfg, 0, x.device)
+    _run("inpc_group_norm_forward", x, C.byref(cfg), x.data_ptr(), _address(weight), _address(bias), y.data_ptr(),
+         moments.data_ptr(), _address(workspace), size)
+    return y, x, moments, cfg
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, groups: int, eps: float,
-                activation: int, p: float, seed: int, seed_tensor: torch.Tensor | None, offset: int) -> torch.Tensor:
-        x, image_stride, pixel_stride = _channels_last(x)
-        n, c, h, w = x.shape
-        param_dtype = next((_DTYPES[t.dtype] for t in (weight, bias) if t is not None), _lib.DTYPE_F32)
-        cfg = _lib.GroupNormConfig(n, h * w, c, groups, _DTYPES[x.dtype], param_dtype, activation, eps, image_stride,
-                                   pixel_stride, 0, 0, p, seed, None if seed_tensor is None else seed_tensor.data_ptr(), offset)
-        y = _dense(x)
-        moments = torch.empty((n * groups, 2), dtype=torch.float32, device=x.device)
-        with _on_device_of(x):
-            workspace, size = _workspace(cfg, x.device)
-            _lib.check(_lib.lib().inpc_group_norm_forward(C.byref(cfg), _lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias),
-                                                          _lib.ptr(y), _lib.ptr(moments), _lib.ptr(workspace), size,
-                                                          _lib.current_stream()), "inpc_group_norm_forward")
-        ctx.cfg = cfg
-        ctx.save_for_backward(x, weight, bias, moments, seed_tensor)
+    def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, options: tuple) -> torch.Tensor:
+        y, x, moments, ctx.cfg = _group_norm_call(x, weight, bias, *options)
+        ctx.save_for_backward(x, weight, bias, moments, options[5])   # the last: a seed on the GPU, which torch watches over
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):
-        x, weight, bias, moments, seed_tensor = ctx.saved_tensors
-        cfg = _lib.GroupNormConfig.from_buffer_copy(ctx.cfg)
+        x, weight, bias, moments, _ = ctx.saved_tensors
+        cfg = _lib.GroupNormConfig.from_buffer_copy(ctx.cfg)   # two backward passes of one forward pass may run at once
         grad, cfg.grad_image_stride, cfg.grad_pixel_stride = _channels_last(grad)
-        need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
-        zeros = torch.zeros_like if x.numel() == 0 else torch.empty_like
+        need_x, need_weight, need_bias, _ = ctx.needs_input_grad
+        new = torch.empty_like if x.numel() else torch.zeros_like
         dx = _dense(x) if need_x else None
-        dweight = zeros(weight, memory_format=torch.contiguous_format) if need_weight else None
-        dbias = zeros(bias, memory_format=torch.contiguous_format) if need_bias else None
-        with _on_device_of(x):
-            workspace, size = _workspace(cfg, x.device)
-            _lib.check(_lib.lib().inpc_group_norm_backward(C.byref(cfg), _lib.ptr(grad), _lib.ptr(x), _lib.ptr(weight),
-                                                           _lib.ptr(bias), _lib.ptr(moments), _lib.ptr(dx), _lib.ptr(dweight),
-                                                           _lib.ptr(dbias), _lib.ptr(workspace), size, _lib.current_stream()),
-                       "inpc_group_norm_backward")
-        return dx, dweight, dbias, None, None, None, None, None, None, None
+        dweight = new(weight) if need_weight else None
+        dbias = new(bias) if need_bias else None
+        workspace, size = _workspace(cfg, 1, x.device)
+        _run("inpc_group_norm_backward", x, C.byref(cfg), grad.data_ptr(), x.data_ptr(), _address(weight), _address(bias),
+             moments.data_ptr(), _address(dx), _address(dweight), _address(dbias), _address(workspace), size)
+        return dx, dweight, dbias, None
 
 
 def group_norm(input: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -225,4 +234,8 @@ def group_norm(input: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     p = _require_probability(dropout_p, "dropout_p") if training else 0.0
     seed, seed_tensor, offset = _require_seed(seed, offset, input.device) if p > 0.0 else (0, None, 0)
     weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
-    return _GroupNorm.apply(input, weight, bias, num_groups, float(eps), _ACTIVATIONS[activation], p, seed, seed_tensor, offset)
+    options = num_groups, float(eps), _ACTIVATIONS[activation], p, seed, seed_tensor, offset
+    if torch.is_grad_enabled() and (input.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _GroupNorm.apply(input, weight, bias, options)
+    return _group_norm_call(input, weight, bias, *options)[0]

@@ -190,6 +190,25 @@ def test_group_norm(gpu, shape, dtype):
     check(*make_case(*size, dtype, sum(shape)), groups)
 
 
+# maps whose groups are too large for one block each: slabs of pixels in one launch, the result in a second
+SPLIT_SHAPES = [
+    (1, 8, 150, 161, 1, "fp32", "none", 0.0),
+    (1, 8, 150, 161, 1, "bf16", "silu", 0.0),
+    (2, 24, 120, 95, 3, "fp16", "gelu", 0.25),      # columns that are no power of two
+    (2, 24, 120, 95, 3, "fp32", "silu", 0.25),
+    (3, 6, 210, 113, 2, "bf16", "silu", 0.5),       # vectors of two, 170 rows to a block
+    (1, 40, 120, 75, 5, "fp32", "relu", 0.0),
+    (1, 33, 200, 200, 33, "fp32", "silu", 0.1),     # single elements, more slab sums than every block adds up itself
+    (1, 640, 41, 13, 2, "fp16", "none", 0.0),       # 80 columns, 320 channels to a group
+]
+
+
+@pytest.mark.parametrize("shape", SPLIT_SHAPES, ids=str)
+def test_group_norm_of_large_groups(gpu, shape):
+    *size, groups, dtype, act, p = shape
+    check(*make_case(*size, dtype, sum(size)), groups, act, p=p, seed=19)
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
 @pytest.mark.parametrize("p", [0.0, 0.35])

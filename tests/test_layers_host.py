@@ -77,11 +77,11 @@ def test_refused_configurations(changes, code, word):
 def test_refused_pointers_and_workspaces():
     lib = _lib.lib()
     cfg = config()
-    size = lib.inpc_group_norm_workspace_bytes(C.byref(cfg))
+    size = lib.inpc_group_norm_workspace_bytes(C.byref(cfg), 0)
     fake = (C.c_char * 256)()
     p = C.c_void_p((C.addressof(fake) + 15) & ~15)
-    assert lib.inpc_group_norm_workspace_bytes(C.byref(config(groups=3))) == 0
-    assert lib.inpc_group_norm_workspace_bytes(None) == 0
+    assert lib.inpc_group_norm_workspace_bytes(C.byref(config(groups=3)), 0) == 0
+    assert lib.inpc_group_norm_workspace_bytes(None, 1) == 0
     assert lib.inpc_group_norm_forward(None, p, None, None, p, p, p, size, None) == -1
     for args in ((None, None, None, p, p), (p, None, None, None, p), (p, None, None, p, None)):
         assert lib.inpc_group_norm_forward(C.byref(cfg), *args, p, size, None) == -1
@@ -92,12 +92,18 @@ def test_refused_pointers_and_workspaces():
     assert lib.inpc_group_norm_forward(C.byref(empty), None, None, None, None, None, None, 0, None) == 0
     assert lib.inpc_group_norm_backward(C.byref(cfg), None, None, None, None, None, None, None, None, None, 0, None) == 0
     large = config(n_pixels=1_000_000, input_image_stride=8_000_000, grad_image_stride=8_000_000)
-    size = lib.inpc_group_norm_workspace_bytes(C.byref(large))
-    assert size > 0
-    for workspace, held in ((p, size - 1), (None, size), (C.c_void_p(p.value + 4), size)):
-        assert lib.inpc_group_norm_forward(C.byref(large), p, None, None, p, p, workspace, held, None) == -2
-        assert lib.inpc_group_norm_backward(C.byref(large), p, p, None, None, p, p, None, None, workspace, held, None) == -2
-        assert b"workspace" in lib.inpc_last_error()
+    sizes = [lib.inpc_group_norm_workspace_bytes(C.byref(large), backward) for backward in (0, 1)]
+    assert 0 < sizes[0] < sizes[1]
+    for backward, size in enumerate(sizes):
+        for workspace, held in ((p, size - 1), (None, size), (C.c_void_p(p.value + 4), size)):
+            if backward:
+                rc = lib.inpc_group_norm_backward(C.byref(large), p, p, None, None, p, p, None, None, workspace, held, None)
+            else:
+                rc = lib.inpc_group_norm_forward(C.byref(large), p, None, None, p, p, workspace, held, None)
+            assert rc == -2 and b"workspace" in lib.inpc_last_error()
+    # small maps need none, except to add up the parameters' gradients of several images
+    assert lib.inpc_group_norm_workspace_bytes(C.byref(cfg), 0) == lib.inpc_group_norm_workspace_bytes(C.byref(cfg), 1) == 0
+    assert lib.inpc_group_norm_workspace_bytes(C.byref(config(n_images=3)), 1) == 3 * 8 * 8
     assert lib.inpc_dropout(None, p, 4, 0, 0.5, 1, None, 0, None) == -1
     assert lib.inpc_dropout(p, None, 4, 0, 0.5, 1, None, 0, None) == -1
     assert lib.inpc_dropout(p, p, 4, 3, 0.5, 1, None, 0, None) == -3
