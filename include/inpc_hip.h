@@ -581,7 +581,7 @@ int inpc_cauchy_loss_backward(const float* grad, const float* input, const float
 /* Group norm over channels-last feature maps: n_images images of n_pixels pixels of `channels` adjacent
  * values, the channels split into `groups` equal groups. Strides are in elements: from image to image and
  * from pixel to pixel of the input (a slice of the channels of a wider map is an input like any other) and
- * of the output's gradient (backward only); output and input gradient are dense. */
+ * of the output's gradient (backward only); pixel strides are below 2^19; output and input gradient are dense. */
 #define INPC_GROUP_NORM_MAX_CHANNELS 65536u
 typedef struct inpc_group_norm_config {
     uint32_t n_images, n_pixels; /* fewer than 2^30 pixels per image                              */

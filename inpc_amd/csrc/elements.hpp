@@ -105,6 +105,23 @@ __device__ __forceinline__ float load_element(const void* base, int32_t dtype, s
     const uint32_t bits = ((const uint16_t*)base)[i];
     return dtype == INPC_DTYPE_F16 ? f16_value(bits) : bf16_value(bits);
 }
+// V neighbouring ones, `otherwise` where there are none. The type is asked once, so that all loads are on their way together.
+template <int V>
+__device__ __forceinline__ void load_elements(const void* base, int32_t dtype, size_t first, float otherwise, float (&v)[V]) {
+    if (!base) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = otherwise;
+    } else if (dtype == INPC_DTYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = ((const float*)base)[first + j];
+    } else {
+        uint16_t bits[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) bits[j] = ((const uint16_t*)base)[first + j];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = dtype == INPC_DTYPE_F16 ? f16_value(bits[j]) : bf16_value(bits[j]);
+    }
+}
 __device__ __forceinline__ void store_element(void* base, int32_t dtype, size_t i, float v) {
     if (dtype == INPC_DTYPE_F32) ((float*)base)[i] = v;
     else ((uint16_t*)base)[i] = (uint16_t)(dtype == INPC_DTYPE_F16 ? f16_bits(v) : bf16_bits(v));

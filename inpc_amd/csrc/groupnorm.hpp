@@ -6,27 +6,29 @@
 //   dx = (weight * dz - A - xhat * B) / sqrt(var + eps), A and B the group's means of weight * dz and weight * dz * xhat
 //
 // Two forms. "single": a block per (image, group) does everything in one launch, from registers where the group fits them;
-// for maps whose launches cost more than their bytes. "split": a block per run of pixels (a slab) of an image and all
-// of its channels, so that it reads whole runs of memory; one launch writes each slab's sums, the next adds
-// them up at the start of every block and applies. In both a thread keeps one vector of channels (16 bytes where channel
-// counts, strides and pointers allow). Sums are fp32 in an order that depends on sizes and alignments alone (no atomics);
-// deviations are taken from a mean, never squares from squares, so that nothing cancels however far the values are from 0.
+// for maps whose launches cost more than their bytes. "split": a block per run of pixels (a slab) of an image, all channels
+// of it wide, so that it reads whole runs of memory; one launch writes each slab's sums, the next adds them up at the
+// start of every block and applies. In both a thread keeps one vector of channels (16 bytes where channel counts, strides
+// and pointers allow). Sums are fp32 in an order that depends on sizes and alignments alone (no atomics); deviations are
+// taken from a value of the data, so that nothing cancels however far the values are from 0.
 #pragma once
 
 #include <algorithm>
+#include <utility>
 
 #include "elements.hpp"
 
 namespace inpc {
 namespace norm {
 
-constexpr int kMaxThreads = 1024;        // of the single form
-constexpr int kMaxThreadsBackward = 512; // ... whose threads need more registers here
-constexpr int kHeld = 8;                 // vectors of x, and in the backward pass of dy, a thread of it keeps in registers
+constexpr int kMaxThreads = 512;         // of the single form
 constexpr int kThreads = 512;            // of the split form
-constexpr int kUnroll = 4;               // pixels a thread of it has in flight
-constexpr uint32_t kFillBlocks = 512;    // blocks that fill the chip: two per compute unit
-constexpr uint32_t kFoldedSums = 8192;   // slab sums of an image up to which every block adds them up itself
+constexpr int kUnroll = 4;               // vectors a thread has in flight
+constexpr int kUnrollBackward = 2;       // ... of x and of dy each
+constexpr uint32_t kSumBlocks = 512;     // of the split form: two on each compute unit
+constexpr uint32_t kApplyBlocks = 1024;  // ... where sums need not be added up by every block
+constexpr uint32_t kFoldedSums = 4096;   // slab sums of a tile of an image up to which they are
+constexpr uint32_t kTileGroups = 32;     // groups of a tile at most
 constexpr uint32_t kParameterColumns = 32;
 
 struct Shape {
@@ -34,21 +36,33 @@ struct Shape {
     uint64_t g_image, g_pixel;   // of the gradient of y
     uint32_t n, pixels, channels, groups, per_group;
     uint32_t columns, rows;      // threads of a block: vectors side by side, pixels at once
-    uint32_t slabs, slab_pixels; // split form, per image
+    uint32_t tiles, tile_groups; // split form: tiles of channels, and whole groups in each (fewer in the last)
+    uint32_t slabs, slab_pixels; // ... and runs of pixels of each tile of an image
     int32_t activation, param_dtype;
     float eps;
 };
 
+// f(0), ..., f(N - 1) written out with constant arguments: an array indexed by them stays in registers, which a loop that the
+// compiler only unrolls late does not guarantee.
+template <typename F, int... K>
+__device__ __forceinline__ void written_out(F& f, std::integer_sequence<int, K...>) {
+    (f(std::integral_constant<int, K>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void written_out(F f) {
+    written_out(f, std::make_integer_sequence<int, N>{});
+}
+
 // ---- sums over a block -----------------------------------------------------------------------------------------------
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// Sum over `lanes` neighbouring lanes (a power of two), in all of them
+__device__ __forceinline__ float lanes_sum(float v, uint32_t lanes) {
+    for (uint32_t o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, (int)o, 64);
     return v;
 }
 
 // The sum of all threads' values, in every thread. `lds`: one float per wave; free again when the next barrier has passed.
 __device__ __forceinline__ float block_sum(float v, float* lds) {
-    v = wave_sum(v);
+    v = lanes_sum(v, 64);
     const uint32_t waves = blockDim.x / 64u;
     __syncthreads();
     if (lane_id() == 0) lds[threadIdx.x / 64u] = v;
@@ -58,57 +72,39 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
     return total;
 }
 
-// Adds N values per thread over the threads of a column (thread = row * columns + column; threads beyond rows * columns
-// bring zeros). Returns where the totals lie in LDS, [column][N], for every thread to read until the next call.
-// `lds` holds blockDim.x * N + 32 * N floats.
-template <int N>
-__device__ __forceinline__ const float* column_sums(const float (&values)[N], uint32_t columns, uint32_t rows, float* lds) {
-    const uint32_t t = threadIdx.x;
-    __syncthreads();
-    if (columns <= 32u && (columns & (columns - 1u)) == 0u) {
-        // the lanes of a wave first, then the waves
-        float v[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = values[j];
-        for (uint32_t o = columns; o < 64u; o <<= 1)
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] += __shfl_xor(v[j], (int)o, 64);
-        const uint32_t waves = blockDim.x / 64u, width = columns * N;
-        if (lane_id() < columns)
-#pragma unroll
-            for (int j = 0; j < N; ++j) lds[(t / 64u) * width + lane_id() * N + j] = v[j];
-        __syncthreads();
-        float* total = lds + blockDim.x * N;
-        for (uint32_t i = t; i < width; i += blockDim.x) {
-            float sum = 0.0f;
-            for (uint32_t w = 0; w < waves; ++w) sum += lds[w * width + i];
-            total[i] = sum;
-        }
-        __syncthreads();
-        return total;
-    }
-#pragma unroll
-    for (int j = 0; j < N; ++j) lds[t * N + j] = values[j];
-    const uint32_t row = t / columns;
-    uint32_t half = 1;
-    while (half < rows) half <<= 1;
-    for (half >>= 1; half > 0; half >>= 1) {
-        __syncthreads();
-        if (row < half && row + half < rows)
-#pragma unroll
-            for (int j = 0; j < N; ++j) lds[t * N + j] += lds[(t + half * columns) * N + j];
-    }
-    __syncthreads();
-    return lds;
+// The largest power of two of lanes, up to a wave, that `parts` parts of a block can have each
+__device__ __forceinline__ uint32_t lanes_for(uint32_t parts) {
+    uint32_t lanes = 64;
+    while (lanes > 1 && lanes * parts > blockDim.x) lanes >>= 1;
+    return lanes;
 }
 
-// Two sets of values merged: counts na and nb, means, sums of squared deviations (Chan, Golub, LeVeque 1979).
-__device__ __forceinline__ void merge_moments(float& na, float& mean, float& m2, float nb, float mean_b, float m2_b) {
-    if (nb == 0.0f) return;
-    const float n = na + nb, d = mean_b - mean, share = nb / n;
-    mean = fmaf(d, share, mean);
-    m2 += fmaf(d * d, na * share, m2_b);
-    na = n;
+// Adds V values per thread over the threads of a column (thread = row * columns + column). Returns where the totals lie in LDS,
+// [column][V], for every thread to read until the next barrier after the next call. `lds` holds column_floats<V>(blockDim.x).
+template <int V>
+constexpr size_t column_floats(size_t threads) { return threads * (V + 1) + threads * V / 2; }
+
+template <int V>
+__device__ __forceinline__ float* column_sums(const float (&v)[V], uint32_t columns, uint32_t rows, float* lds) {
+    const uint32_t width = columns * V, stride = width + 1, row = threadIdx.x / columns;   // an odd stride: no bank twice
+    __syncthreads();
+    if (row < rows)
+#pragma unroll
+        for (int j = 0; j < V; ++j) lds[row * stride + threadIdx.x % columns * V + j] = v[j];
+    __syncthreads();
+    if (rows == 1) return lds;
+    float* total = lds + blockDim.x * (V + 1);
+    const uint32_t lanes = lanes_for(width), lane = threadIdx.x % lanes;
+    for (uint32_t base = 0; base < width; base += blockDim.x / lanes) {
+        const uint32_t channel = base + threadIdx.x / lanes;
+        float sum = 0.0f;
+        if (channel < width)
+            for (uint32_t r = lane; r < rows; r += lanes) sum += lds[r * stride + channel];
+        sum = lanes_sum(sum, lanes);
+        if (lane == 0 && channel < width) total[channel] = sum;
+    }
+    __syncthreads();
+    return total;
 }
 
 // ---- activations -----------------------------------------------------------------------------------------------------
@@ -148,66 +144,184 @@ __device__ __forceinline__ void activate_backward(int32_t activation, const floa
 }
 
 // ---- one vector ------------------------------------------------------------------------------------------------------
-template <int V>
-struct Parameters {
-    float weight[V], bias[V];
+// A vector's V channels are Q slots of channels that share a group: 1 where the vector lies in one group, 2 where it lies in
+// two of half a vector each, else V. z = (x - mean) * scale + bias, scale = weight / sqrt(var + eps).
+template <int V, int Q>
+struct Affine {
+    float mean[Q], rstd[Q], scale[V], bias[V];
 };
-template <int V>
-__device__ __forceinline__ Parameters<V> load_parameters(const Shape& s, const void* weight, const void* bias, uint32_t channel) {
-    Parameters<V> p;
+
+// `moments`: of the group of channel `first`, the vector's first channel being `channel`
+template <int V, int Q>
+__device__ __forceinline__ Affine<V, Q> load_affine(const Shape& s, const float2* moments, uint32_t first, uint32_t channel,
+                                                    const void* weight, const void* bias) {
+    Affine<V, Q> a;
+    load_elements<V>(weight, s.param_dtype, channel, 1.0f, a.scale);
+    load_elements<V>(bias, s.param_dtype, channel, 0.0f, a.bias);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        p.weight[j] = weight ? load_element(weight, s.param_dtype, channel + j) : 1.0f;
-        p.bias[j] = bias ? load_element(bias, s.param_dtype, channel + j) : 0.0f;
+    for (int q = 0; q < Q; ++q) {
+        const float2 m = moments[(channel - first + q * (V / Q)) / s.per_group];
+        a.mean[q] = m.x;
+        a.rstd[q] = m.y;
     }
-    return p;
+#pragma unroll
+    for (int j = 0; j < V; ++j) a.scale[j] *= a.rstd[j / (V / Q)];
+    return a;
 }
 
-// The moments of a vector's channels: one pair where all of them lie in one group (M = 1), else a pair each (M = V).
-template <int M>
-struct Moments {
-    float mean[M], rstd[M];
+// A thread's vectors in one run of pixels of a feature map, `rows` pixels apart: vector k at base + k * step + lane. All but
+// `lane` is the same for the whole block, so that an address costs scalar arithmetic and one register per thread.
+struct Rows {
+    char* base;
+    uint64_t step;   // bytes
+    uint32_t lane;   // bytes
 };
+// `first`: the element that the run's first pixel and the block's first channel make
+template <int D, int V>
+__device__ __forceinline__ Rows rows_of(const void* map, uint64_t first, uint64_t pixel_stride, const Shape& s) {
+    return Rows{(char*)map + first * kElementBytes<D>, s.rows * pixel_stride * kElementBytes<D>,
+                (uint32_t)((threadIdx.x / s.columns * (uint32_t)pixel_stride + threadIdx.x % s.columns * V) * kElementBytes<D>)};
+}
+template <int D, int V>
+__device__ __forceinline__ PackedVector<D, V> load_row(const Rows& m, uint32_t k, uint32_t skip = 0) {
+    return *(const PackedVector<D, V>*)(m.base + k * m.step + (m.lane + skip * kElementBytes<D>));
+}
 
-template <int D, int V, int M>
-__device__ __forceinline__ void apply_vector(const Shape& s, const Dropout& d, uint64_t seed, const Moments<M>& m,
-                                             const Parameters<V>& p, const PackedVector<D, V>& packed, void* y, size_t at) {
+template <int D, int V>
+__device__ __forceinline__ void store_row(const Rows& m, uint32_t k, uint32_t skip, const float (&v)[V]) {
+    *(PackedVector<D, V>*)(m.base + k * m.step + (m.lane + skip * kElementBytes<D>)) = pack<D, V>(v);
+}
+
+// The same for element numbers: of the result, which is dense
+struct Numbers {
+    uint64_t first;
+    uint32_t step, lane;
+};
+template <int V>
+__device__ __forceinline__ Numbers numbers_of(uint64_t first, const Shape& s) {
+    return Numbers{first, s.rows * s.channels, threadIdx.x / s.columns * s.channels + threadIdx.x % s.columns * V};
+}
+__device__ __forceinline__ uint64_t number_of(const Numbers& n, uint32_t k, uint32_t skip = 0) {
+    return n.first + (uint64_t)k * n.step + (n.lane + skip);
+}
+
+template <int D, int V, int Q>
+__device__ __forceinline__ void apply_vector(const Shape& s, const Dropout& d, uint64_t seed, const Affine<V, Q>& a,
+                                             const PackedVector<D, V>& packed, const Rows& y, const Numbers& numbers,
+                                             uint32_t k, uint32_t skip = 0) {
     float v[V];
     unpack<D, V>(packed, v);
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = fmaf((v[j] - m.mean[j % M]) * m.rstd[j % M], p.weight[j], p.bias[j]);
+    for (int j = 0; j < V; ++j) v[j] = fmaf(v[j] - a.mean[j / (V / Q)], a.scale[j], a.bias[j]);
     activate<V>(s.activation, v);
-    if (d.on) dropout_apply<V>(d, seed, at, v);
-    store_vector<D, V>(y, at, v);
+    if (d.on) dropout_apply<V>(d, seed, number_of(numbers, k, skip), v);
+    store_row<D, V>(y, k, skip, v);
 }
 
-// xhat in v and dz in g
-template <int D, int V, int M>
-__device__ __forceinline__ void gradient_vector(const Shape& s, const Dropout& d, uint64_t seed, const Moments<M>& m,
-                                                const Parameters<V>& p, const PackedVector<D, V>& px, const PackedVector<D, V>& pg,
-                                                size_t at, float (&v)[V], float (&g)[V]) {
+// x - mean in v and dz in g
+template <int D, int V, int Q>
+__device__ __forceinline__ void gradient_vector(const Shape& s, const Dropout& d, uint64_t seed, const Affine<V, Q>& a,
+                                                const PackedVector<D, V>& px, const PackedVector<D, V>& pg, uint64_t number,
+                                                float (&v)[V], float (&g)[V]) {
     float z[V];
     unpack<D, V>(px, v);
     unpack<D, V>(pg, g);
-    if (d.on) dropout_apply<V>(d, seed, at, g);
+    if (d.on) dropout_apply<V>(d, seed, number, g);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        v[j] = (v[j] - m.mean[j % M]) * m.rstd[j % M];
-        z[j] = fmaf(v[j], p.weight[j], p.bias[j]);
+        v[j] -= a.mean[j / (V / Q)];
+        z[j] = fmaf(v[j], a.scale[j], a.bias[j]);
     }
     activate_backward<V>(s.activation, z, g);
 }
 
-template <int D, int V, int M>
-__device__ __forceinline__ void input_gradient_vector(const Shape& s, const Dropout& d, uint64_t seed, const Moments<M>& m,
-                                                      const float (&mean_a)[M], const float (&mean_b)[M], const Parameters<V>& p,
-                                                      const PackedVector<D, V>& px, const PackedVector<D, V>& pg, void* dx, size_t at) {
+// dx = dz * scale - k1 - (x - mean) * k2, k1 = A / sqrt(var + eps), k2 = B / (var + eps)
+template <int D, int V, int Q>
+__device__ __forceinline__ void input_gradient_vector(const Shape& s, const Dropout& d, uint64_t seed, const Affine<V, Q>& a,
+                                                      const float (&k1)[Q], const float (&k2)[Q], const PackedVector<D, V>& px,
+                                                      const PackedVector<D, V>& pg, const Rows& dx, const Numbers& numbers,
+                                                      uint32_t k, uint32_t skip = 0) {
     float v[V], g[V];
-    gradient_vector<D, V, M>(s, d, seed, m, p, px, pg, at, v, g);
+    gradient_vector<D, V, Q>(s, d, seed, a, px, pg, number_of(numbers, k, skip), v, g);
 #pragma unroll
-    for (int j = 0; j < V; ++j) g[j] = (fmaf(g[j], p.weight[j], -mean_a[j % M]) - v[j] * mean_b[j % M]) * m.rstd[j % M];
-    store_vector<D, V>(dx, at, g);
+    for (int j = 0; j < V; ++j) g[j] = fmaf(-v[j], k2[j / (V / Q)], fmaf(g[j], a.scale[j], -k1[j / (V / Q)]));
+    store_row<D, V>(dx, k, skip, g);
 }
+
+// The same rows `skip` elements further
+template <int D>
+__device__ __forceinline__ Rows shifted(Rows m, uint32_t skip) {
+    m.lane += skip * kElementBytes<D>;
+    return m;
+}
+
+// f(k, vector k of the map, or of both) for all vectors that a thread has in a run of `size` pixels: N at a time, loaded before the first is used. `k` is
+// the same for the whole block.
+template <int D, int V, int N, typename F>
+__device__ __forceinline__ void stream(const Rows& x, uint32_t rows, uint32_t size, uint32_t row, F f) {
+    if (row >= size) return;
+    const uint32_t whole = size / rows, rest = size % rows;
+    uint32_t k = 0;
+    for (; k + N <= whole; k += N) {
+        PackedVector<D, V> packed[N];
+        written_out<N>([&](auto i) { packed[i] = load_row<D, V>(x, k + i); });
+        written_out<N>([&](auto i) { f(k + i, packed[i]); });
+    }
+    for (; k < whole; ++k) f(k, load_row<D, V>(x, k));
+    if (row < rest) f(whole, load_row<D, V>(x, whole));
+}
+template <int D, int V, int N, typename F>
+__device__ __forceinline__ void stream(const Rows& x, const Rows& g, uint32_t rows, uint32_t size, uint32_t row, F f) {
+    if (row >= size) return;
+    const uint32_t whole = size / rows, rest = size % rows;
+    uint32_t k = 0;
+    for (; k + N <= whole; k += N) {
+        PackedVector<D, V> px[N], pg[N];
+        written_out<N>([&](auto i) {
+            px[i] = load_row<D, V>(x, k + i);
+            pg[i] = load_row<D, V>(g, k + i);
+        });
+        written_out<N>([&](auto i) { f(k + i, px[i], pg[i]); });
+    }
+    for (; k < whole; ++k) f(k, load_row<D, V>(x, k), load_row<D, V>(g, k));
+    if (row < rest) f(whole, load_row<D, V>(x, whole), load_row<D, V>(g, whole));
+}
+
+// A thread's sums of differences from its first value, for each slot of its vectors. N values with a common pivot that is one of
+// them: the pivot's squared distance from the group's mean is at most the group's sum of squared deviations, so that what cancels
+// in s2 - s1^2 / N costs at most a factor of N (some hundred) in the last place.
+template <int V, int Q>
+struct Differences {
+    float pivot[Q], s1[Q], s2[Q];
+    __device__ __forceinline__ Differences() {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) pivot[q] = s1[q] = s2[q] = 0.0f;
+    }
+    __device__ __forceinline__ void add(const float (&v)[V], bool first) {
+        constexpr int W = V / Q;   // channels of a slot
+        if (first)
+#pragma unroll
+            for (int q = 0; q < Q; ++q) pivot[q] = v[q * W];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            float a[2] = {0.0f, 0.0f}, b[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float d = v[q * W + j] - pivot[q];
+                a[j & 1] += d;
+                b[j & 1] = fmaf(d, d, b[j & 1]);
+            }
+            s1[q] += a[0] + a[1];
+            s2[q] += b[0] + b[1];
+        }
+    }
+    // with n values: their sum, and the sum of their squared deviations from `mean`
+    __device__ __forceinline__ float sum(int q, float n) const { return fmaf(n, pivot[q], s1[q]); }
+    __device__ __forceinline__ float deviations(int q, float n, float share, float mean) const {   // share: 1 / n, or 0
+        const float own = s1[q] * share, d = pivot[q] + own - mean;
+        return fmaf(n * d, d, fmaxf(fmaf(-s1[q], own, s2[q]), 0.0f));
+    }
+};
 
 // ---- the single form -------------------------------------------------------------------------------------------------
 // Blocks go to the eight dies in turn: neighbouring (image, group) pairs, which share cache lines, go to one die.
@@ -222,540 +336,413 @@ __global__ void __launch_bounds__(kMaxThreads) k_single(const void* __restrict__
                                                         float2* __restrict__ moments, Shape s, Dropout d) {
     __shared__ float lds[kMaxThreads / 64];
     const uint32_t b = swizzled_block(), image = b / s.groups, first = b % s.groups * s.per_group;
-    const uint32_t column = threadIdx.x % s.columns, row = threadIdx.x / s.columns, vectors = s.per_group / V;
-    const size_t base = (size_t)image * s.x_image + first, out = (size_t)image * s.pixels * s.channels + first;
-    const float count = (float)s.pixels * (float)s.per_group;
-    const bool held = s.columns == vectors && s.pixels <= s.rows * kHeld, active = row < s.rows;
-    PackedVector<D, V> px[kHeld];
-    Moments<1> m;
-    float variance;
-    if (held) {
-        // the whole group is in the block's registers: its mean, then the squares of the deviations from that
-        float sum = 0.0f, squares = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kHeld; ++k)
-            if (active && row + k * s.rows < s.pixels) px[k] = load_packed<D, V>(x, base + (size_t)(row + k * s.rows) * s.x_pixel + column * V);
-#pragma unroll
-        for (int k = 0; k < kHeld; ++k)
-            if (active && row + k * s.rows < s.pixels) {
-                float v[V];
-                unpack<D, V>(px[k], v);
-#pragma unroll
-                for (int j = 0; j < V; ++j) sum += v[j];
-            }
-        m.mean[0] = block_sum(sum, lds) / count;
-#pragma unroll
-        for (int k = 0; k < kHeld; ++k)
-            if (active && row + k * s.rows < s.pixels) {
-                float v[V];
-                unpack<D, V>(px[k], v);
-#pragma unroll
-                for (int j = 0; j < V; ++j) squares = fmaf(v[j] - m.mean[0], v[j] - m.mean[0], squares);
-            }
-        variance = block_sum(squares, lds) / count;
-    } else {
-        // a thread's values vector by vector, then the threads
-        float n = 0.0f, mean = 0.0f, m2 = 0.0f;
-        if (active)
-            for (uint32_t c = column; c < vectors; c += s.columns)
-                for (uint32_t r = row; r < s.pixels; r += s.rows) {
-                    float v[V], vector_mean = 0.0f, vector_m2 = 0.0f;
-                    load_vector<D, V>(x, base + (size_t)r * s.x_pixel + c * V, v);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) vector_mean += v[j];
-                    vector_mean *= 1.0f / V;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) vector_m2 = fmaf(v[j] - vector_mean, v[j] - vector_mean, vector_m2);
-                    merge_moments(n, mean, m2, (float)V, vector_mean, vector_m2);
-                }
-        m.mean[0] = block_sum(n * mean, lds) / count;
-        variance = block_sum(fmaf(n * (mean - m.mean[0]), mean - m.mean[0], m2), lds) / count;
-    }
-    m.rstd[0] = 1.0f / sqrtf(variance + s.eps);
-    if (threadIdx.x == 0) moments[b] = make_float2(m.mean[0], m.rstd[0]);
-    if (!active) return;
+    const uint32_t column = threadIdx.x % s.columns, vectors = s.per_group / V;
+    const uint32_t row = threadIdx.x / s.columns < s.rows ? threadIdx.x / s.columns : 0xFFFFFFFFu;
+    const uint64_t out = (uint64_t)image * s.pixels * s.channels + first;
+    const Rows rx = rows_of<D, V>(x, image * s.x_image + first, s.x_pixel, s), ry = rows_of<D, V>(y, out, s.channels, s);
+    Differences<V, 1> sums;
+    uint32_t count = 0;
+    for (uint32_t c = column; c < vectors; c += s.columns)
+        stream<D, V, kUnroll>(shifted<D>(rx, (c - column) * V), s.rows, s.pixels, row, [&](uint32_t, const PackedVector<D, V>& packed) {
+            float v[V];
+            unpack<D, V>(packed, v);
+            sums.add(v, count == 0);
+            count += V;
+        });
+    const float n = (float)count, share = count ? 1.0f / n : 0.0f, all = (float)s.pixels * (float)s.per_group;
+    const float mean = block_sum(sums.sum(0, n), lds) / all;
+    const float2 m = make_float2(mean, 1.0f / sqrtf(block_sum(sums.deviations(0, n, share, mean), lds) / all + s.eps));
+    if (threadIdx.x == 0) moments[b] = m;
     const uint64_t seed = dropout_seed(d);
-    if (held) {
-        const Parameters<V> p = load_parameters<V>(s, weight, bias, first + column * V);
-#pragma unroll
-        for (int k = 0; k < kHeld; ++k) {
-            const uint32_t r = row + k * s.rows;
-            if (r < s.pixels) apply_vector<D, V, 1>(s, d, seed, m, p, px[k], y, out + (size_t)r * s.channels + column * V);
-        }
-        return;
-    }
+    const Numbers numbers = numbers_of<V>(out, s);
     for (uint32_t c = column; c < vectors; c += s.columns) {
-        const Parameters<V> p = load_parameters<V>(s, weight, bias, first + c * V);
-        for (uint32_t r = row; r < s.pixels; r += s.rows)
-            apply_vector<D, V, 1>(s, d, seed, m, p, load_packed<D, V>(x, base + (size_t)r * s.x_pixel + c * V), y,
-                                  out + (size_t)r * s.channels + c * V);
+        const uint32_t skip = (c - column) * V;
+        const Affine<V, 1> a = load_affine<V, 1>(s, &m, first + c * V, first + c * V, weight, bias);
+        stream<D, V, kUnroll>(shifted<D>(rx, skip), s.rows, s.pixels, row, [&](uint32_t k, const PackedVector<D, V>& packed) {
+            apply_vector<D, V, 1>(s, d, seed, a, packed, ry, numbers, k, skip);
+        });
     }
 }
 
 // With one image dbias and dweight come from here, with more the sums of every (image, channel) do.
 template <int D, int V>
-__global__ void __launch_bounds__(kMaxThreadsBackward) k_single_backward(const void* __restrict__ x, const void* __restrict__ dy,
-                                                                 const float2* __restrict__ moments,
-                                                                 const void* __restrict__ weight, const void* __restrict__ bias,
-                                                                 void* __restrict__ dx, void* __restrict__ dweight,
-                                                                 void* __restrict__ dbias, float2* __restrict__ sums, Shape s,
-                                                                 Dropout d) {
-    INPC_DYNAMIC_LDS(float, lds);   // column_sums of 2 V values per thread
-    __shared__ float waves[kMaxThreadsBackward / 64];
+__global__ void __launch_bounds__(kMaxThreads) k_single_backward(const void* __restrict__ x, const void* __restrict__ dy,
+                                                                 const float2* __restrict__ moments, const void* __restrict__ weight,
+                                                                 const void* __restrict__ bias, void* __restrict__ dx,
+                                                                 void* __restrict__ dweight, void* __restrict__ dbias,
+                                                                 float2* __restrict__ sums, Shape s, Dropout d) {
+    INPC_DYNAMIC_LDS(float, lds);   // column_sums
+    __shared__ float waves[kMaxThreads / 64];
     const uint32_t b = swizzled_block(), image = b / s.groups, first = b % s.groups * s.per_group;
-    const uint32_t column = threadIdx.x % s.columns, row = threadIdx.x / s.columns, vectors = s.per_group / V;
-    const size_t base = (size_t)image * s.x_image + first, gbase = (size_t)image * s.g_image + first;
-    const size_t out = (size_t)image * s.pixels * s.channels + first;
-    const bool held = s.columns == vectors && s.pixels <= s.rows * kHeld, active = row < s.rows;
-    const uint64_t seed = dropout_seed(d);
-    const Moments<1> m{{moments[b].x}, {moments[b].y}};
-    PackedVector<D, V> px[kHeld], pg[kHeld];
+    const uint32_t column = threadIdx.x % s.columns, vectors = s.per_group / V;
+    const uint32_t row = threadIdx.x / s.columns < s.rows ? threadIdx.x / s.columns : 0xFFFFFFFFu;
+    const uint64_t out = (uint64_t)image * s.pixels * s.channels + first, seed = dropout_seed(d);
+    const Rows rx = rows_of<D, V>(x, image * s.x_image + first, s.x_pixel, s), rg = rows_of<D, V>(dy, image * s.g_image + first, s.g_pixel, s);
+    const Numbers numbers = numbers_of<V>(out, s);
+    const float2 m = moments[b];
     float a = 0.0f, bb = 0.0f;
     for (uint32_t tile = 0; tile < vectors; tile += s.columns) {
-        const uint32_t c = tile + column;
-        const bool mine = active && c < vectors;
+        const uint32_t c = tile + column, skip = tile * V;
         float total[2 * V];
 #pragma unroll
         for (int j = 0; j < 2 * V; ++j) total[j] = 0.0f;
-        const auto add = [&](const Parameters<V>& p, const PackedVector<D, V>& vx, const PackedVector<D, V>& vg, uint32_t r) {
-            float v[V], g[V];
-            gradient_vector<D, V, 1>(s, d, seed, m, p, vx, vg, out + (size_t)r * s.channels + c * V, v, g);
+        if (c < vectors) {
+            const Affine<V, 1> affine = load_affine<V, 1>(s, &m, first + c * V, first + c * V, weight, bias);
+            stream<D, V, kUnrollBackward>(shifted<D>(rx, skip), shifted<D>(rg, skip), s.rows, s.pixels, row,
+                                          [&](uint32_t k, const PackedVector<D, V>& px, const PackedVector<D, V>& pg) {
+                                              float v[V], g[V];
+                                              gradient_vector<D, V, 1>(s, d, seed, affine, px, pg, number_of(numbers, k, skip), v, g);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                total[j] += g[j];
-                total[V + j] = fmaf(g[j], v[j], total[V + j]);
-            }
-        };
-        if (mine) {
-            const Parameters<V> p = load_parameters<V>(s, weight, bias, first + c * V);
-            if (held) {
-#pragma unroll
-                for (int k = 0; k < kHeld; ++k) {
-                    const uint32_t r = row + k * s.rows;
-                    if (r < s.pixels) {
-                        px[k] = load_packed<D, V>(x, base + (size_t)r * s.x_pixel + c * V);
-                        pg[k] = load_packed<D, V>(dy, gbase + (size_t)r * s.g_pixel + c * V);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < kHeld; ++k)
-                    if (row + k * s.rows < s.pixels) add(p, px[k], pg[k], row + k * s.rows);
-            } else {
-                for (uint32_t r = row; r < s.pixels; r += s.rows)
-                    add(p, load_packed<D, V>(x, base + (size_t)r * s.x_pixel + c * V),
-                        load_packed<D, V>(dy, gbase + (size_t)r * s.g_pixel + c * V), r);
-            }
+                                              for (int j = 0; j < V; ++j) {
+                                                  total[j] += g[j];
+                                                  total[V + j] = fmaf(g[j], v[j], total[V + j]);
+                                              }
+                                          });
         }
-        const float* columns = column_sums<2 * V>(total, s.columns, s.rows, lds);
         const uint32_t channels = min(s.columns, vectors - tile) * V;
+        const float* totals = column_sums<2 * V>(total, s.columns, s.rows, lds);
         for (uint32_t i = threadIdx.x; i < channels; i += blockDim.x) {
-            const float sum = columns[i / V * (2 * V) + i % V], product = columns[i / V * (2 * V) + V + i % V];
             const uint32_t channel = first + tile * V + i;
+            const float* of_channel = totals + i / V * (2 * V) + i % V;
+            const float2 sum = make_float2(of_channel[0], of_channel[V] * m.y);
             const float w = weight ? load_element(weight, s.param_dtype, channel) : 1.0f;
-            a = fmaf(w, sum, a);
-            bb = fmaf(w, product, bb);
-            if (sums) sums[(size_t)image * s.channels + channel] = make_float2(sum, product);
-            if (dbias) store_element(dbias, s.param_dtype, channel, sum);
-            if (dweight) store_element(dweight, s.param_dtype, channel, product);
+            a = fmaf(w, sum.x, a);
+            bb = fmaf(w, sum.y, bb);
+            if (sums) sums[(size_t)image * s.channels + channel] = sum;
+            if (dbias) store_element(dbias, s.param_dtype, channel, sum.x);
+            if (dweight) store_element(dweight, s.param_dtype, channel, sum.y);
         }
     }
     if (!dx) return;
     const float count = (float)s.pixels * (float)s.per_group;
-    const float mean_a[1] = {block_sum(a, waves) / count}, mean_b[1] = {block_sum(bb, waves) / count};
-    if (!active) return;
+    const float k1[1] = {block_sum(a, waves) / count * m.y}, k2[1] = {block_sum(bb, waves) / count * m.y * m.y};
+    const Rows rdx = rows_of<D, V>(dx, out, s.channels, s);
     for (uint32_t c = column; c < vectors; c += s.columns) {
-        const Parameters<V> p = load_parameters<V>(s, weight, bias, first + c * V);
-        const size_t at = out + c * V;
-        if (held) {
-#pragma unroll
-            for (int k = 0; k < kHeld; ++k) {
-                const uint32_t r = row + k * s.rows;
-                if (r < s.pixels)
-                    input_gradient_vector<D, V, 1>(s, d, seed, m, mean_a, mean_b, p, px[k], pg[k], dx, at + (size_t)r * s.channels);
-            }
-        } else {
-            for (uint32_t r = row; r < s.pixels; r += s.rows)
-                input_gradient_vector<D, V, 1>(s, d, seed, m, mean_a, mean_b, p,
-                                               load_packed<D, V>(x, base + (size_t)r * s.x_pixel + c * V),
-                                               load_packed<D, V>(dy, gbase + (size_t)r * s.g_pixel + c * V), dx,
-                                               at + (size_t)r * s.channels);
-        }
+        const uint32_t skip = (c - column) * V;
+        const Affine<V, 1> affine = load_affine<V, 1>(s, &m, first + c * V, first + c * V, weight, bias);
+        stream<D, V, kUnrollBackward>(shifted<D>(rx, skip), shifted<D>(rg, skip), s.rows, s.pixels, row,
+                                      [&](uint32_t k, const PackedVector<D, V>& px, const PackedVector<D, V>& pg) {
+                                          input_gradient_vector<D, V, 1>(s, d, seed, affine, k1, k2, px, pg, rdx, numbers, k, skip);
+                                      });
     }
 }
 
-// dbias and dweight from `rows` rows of sums, kParameterColumns channels to a block
-__device__ __forceinline__ void add_parameter_gradients(const float2* sums, size_t rows, void* dweight, void* dbias, const Shape& s,
+// dbias and dweight from `rows` rows of channel sums, kParameterColumns channels to a block; `lds`: column_floats<2>
+__device__ __forceinline__ void add_parameter_gradients(const float2* sums, uint32_t rows, void* dweight, void* dbias, const Shape& s,
                                                         uint32_t block, float* lds) {
     const uint32_t channel = block * kParameterColumns + threadIdx.x % kParameterColumns;
     float total[2] = {0.0f, 0.0f};
     if (channel < s.channels)
-        for (size_t r = threadIdx.x / kParameterColumns; r < rows; r += blockDim.x / kParameterColumns) {
-            const float2 v = sums[r * s.channels + channel];
+#pragma unroll 4
+        for (uint32_t r = threadIdx.x / kParameterColumns; r < rows; r += kThreads / kParameterColumns) {
+            const float2 v = sums[(size_t)r * s.channels + channel];
             total[0] += v.x;
             total[1] += v.y;
         }
-    const float* all = column_sums<2>(total, kParameterColumns, blockDim.x / kParameterColumns, lds);
+    const float* all = column_sums<2>(total, kParameterColumns, kThreads / kParameterColumns, lds);
     if (threadIdx.x < kParameterColumns && channel < s.channels) {
         if (dbias) store_element(dbias, s.param_dtype, channel, all[2 * threadIdx.x]);
         if (dweight) store_element(dweight, s.param_dtype, channel, all[2 * threadIdx.x + 1]);
     }
 }
 
-__global__ void __launch_bounds__(kThreads) k_parameter_gradients(const float2* __restrict__ sums, void* __restrict__ dweight,
-                                                                  void* __restrict__ dbias, Shape s) {
-    __shared__ float lds[kThreads * 2 + 64];
-    add_parameter_gradients(sums, s.n, dweight, dbias, s, blockIdx.x, lds);
+__global__ void __launch_bounds__(kThreads) k_parameter_gradients(const float2* __restrict__ sums, uint32_t rows,
+                                                                  void* __restrict__ dweight, void* __restrict__ dbias, Shape s) {
+    __shared__ float lds[column_floats<2>(kThreads)];
+    add_parameter_gradients(sums, rows, dweight, dbias, s, blockIdx.x, lds);
 }
 
 // ---- the split form --------------------------------------------------------------------------------------------------
+// What a block works on: a slab of pixels and a tile of channels (whole groups) of one image
 struct Place {
-    uint32_t image, slab, channel, row, begin, end;
-    bool active;
+    uint32_t image, tile, channel;   // `channel`: the tile's first
+    uint32_t slab, begin, size;
 };
 
-template <int V>
 __device__ __forceinline__ Place place_of(const Shape& s, uint32_t block) {
     Place p;
+    const uint32_t rest = block / s.slabs;
+    p.tile = rest % s.tiles;
+    p.image = rest / s.tiles;
+    p.channel = p.tile * s.tile_groups * s.per_group;
     p.slab = block % s.slabs;
-    p.image = block / s.slabs;
-    p.row = threadIdx.x / s.columns;
-    p.channel = threadIdx.x % s.columns * V;
-    p.active = p.row < s.rows;
     p.begin = p.slab * s.slab_pixels;
-    p.end = min(p.begin + s.slab_pixels, s.pixels);
+    p.size = min(s.slab_pixels, s.pixels - p.begin);
     return p;
 }
 
-// Sums of per_group neighbouring channels, for all groups: totals[channel / V * N + channel % V + which * V] -> sums[group].
-// A power of two of lanes shares a group.
-template <int V, int N>
-__device__ __forceinline__ void group_sums(const float* totals, int which, const Shape& s, float* sums) {
-    uint32_t lanes = 64;
-    while (lanes > 1 && lanes * s.groups > (uint32_t)kThreads) lanes >>= 1;
-    const uint32_t lane = threadIdx.x % lanes;
-    for (uint32_t base = 0; base < s.groups; base += kThreads / lanes) {
-        const uint32_t group = base + threadIdx.x / lanes;
-        float sum = 0.0f;
-        if (group < s.groups)
-            for (uint32_t c = group * s.per_group + lane; c < (group + 1) * s.per_group; c += lanes)
-                sum += totals[c / V * N + c % V + which * V];
-        for (uint32_t o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, (int)o, 64);
-        if (lane == 0 && group < s.groups) sums[group] = sum;
+// ... and its run of pixels in a map
+template <int D, int V>
+__device__ __forceinline__ Rows rows_at(const void* map, const Place& p, uint64_t image_stride, uint64_t pixel_stride, const Shape& s) {
+    return rows_of<D, V>(map, p.image * image_stride + p.begin * pixel_stride + p.channel, pixel_stride, s);
+}
+template <int V>
+__device__ __forceinline__ Numbers numbers_at(const Place& p, const Shape& s) {
+    return numbers_of<V>(((uint64_t)p.image * s.pixels + p.begin) * s.channels + p.channel, s);
+}
+
+__device__ __forceinline__ uint32_t groups_of_tile(const Shape& s, uint32_t tile) {
+    return min(s.tile_groups, s.groups - tile * s.tile_groups);
+}
+
+// Slab sums lie [image][tile][group of the tile][slab]
+__device__ __forceinline__ size_t sums_at(const Shape& s, const Place& p, uint32_t group) {
+    return ((size_t)(p.image * s.tiles + p.tile) * s.tile_groups + group) * s.slabs;
+}
+
+// The calling thread's row in its block; a row of no slab where it has none or its channels are behind the last
+__device__ __forceinline__ uint32_t thread_row(const Shape& s, const Place& p, uint32_t vector) {
+    const uint32_t row = threadIdx.x / s.columns;
+    return row < s.rows && p.channel + threadIdx.x % s.columns * vector < s.channels ? row : 0xFFFFFFFFu;
+}
+
+// Sums over the slots of each group of a tile: values[row * width + slot], `per_group` neighbouring slots of all rows to a group.
+// A power of two of lanes shares a group; at most kTileGroups groups: all at once.
+__device__ __forceinline__ void group_sums(const float* values, uint32_t width, uint32_t rows, uint32_t per_group, uint32_t groups,
+                                           float* sums) {
+    const uint32_t lanes = lanes_for(groups), lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+    float sum = 0.0f;
+    if (group < groups) {
+        const uint32_t count = rows * per_group;
+        if (per_group == 1)
+            for (uint32_t r = lane; r < count; r += lanes) sum += values[r * width + group];
+        else
+            for (uint32_t i = lane; i < count; i += lanes) sum += values[i / per_group * width + group * per_group + i % per_group];
     }
+    sum = lanes_sum(sum, lanes);
+    if (lane == 0 && group < groups) sums[group] = sum;
     __syncthreads();
 }
 
 // {mean, sum of squared deviations} of every (image, slab, group)
-template <int D, int V>
+template <int D, int V, int Q>
 __global__ void __launch_bounds__(kThreads) k_moments(const void* __restrict__ x, float2* __restrict__ partial, Shape s) {
-    INPC_DYNAMIC_LDS(float, lds);   // column_sums, then one float per group
-    float* group = lds + kThreads * V + 32 * V;
-    const Place p = place_of<V>(s, blockIdx.x);
-    float mean[V], m2[V], count = 0.0f, values[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) mean[j] = m2[j] = 0.0f;
-    if (p.active) {
-        const size_t base = (size_t)p.image * s.x_image + p.channel;
-        uint32_t r = p.begin + p.row;
-        for (; r + (kUnroll - 1) * s.rows < p.end; r += kUnroll * s.rows) {
-            PackedVector<D, V> packed[kUnroll];
-            float v[kUnroll][V];
-#pragma unroll
-            for (int k = 0; k < kUnroll; ++k) packed[k] = load_packed<D, V>(x, base + (size_t)(r + k * s.rows) * s.x_pixel);
-#pragma unroll
-            for (int k = 0; k < kUnroll; ++k) unpack<D, V>(packed[k], v[k]);
-            // the moments of these few pixels first, then merged: two passes over registers
-            const float n = count + kUnroll, share = kUnroll / n, weight = count * share;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float sum = v[0][j], squares = 0.0f;
-#pragma unroll
-                for (int k = 1; k < kUnroll; ++k) sum += v[k][j];
-                const float of_these = sum * (1.0f / kUnroll), d = of_these - mean[j];
-#pragma unroll
-                for (int k = 0; k < kUnroll; ++k) squares = fmaf(v[k][j] - of_these, v[k][j] - of_these, squares);
-                mean[j] = fmaf(d, share, mean[j]);
-                m2[j] += fmaf(d * d, weight, squares);
-            }
-            count = n;
-        }
-        for (; r < p.end; r += s.rows) {
-            float v[V];
-            load_vector<D, V>(x, base + (size_t)r * s.x_pixel, v);
-            const float n = count + 1.0f, share = 1.0f / n, weight = count * share;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float d = v[j] - mean[j];
-                mean[j] = fmaf(d, share, mean[j]);
-                m2[j] = fmaf(d * d, weight, m2[j]);
-            }
-            count = n;
-        }
-    }
-    const float in_group = (float)(p.end - p.begin) * (float)s.per_group;
+    constexpr int W = V / Q;   // channels of a slot
+    __shared__ float lds[kThreads * Q];
+    __shared__ float group[kTileGroups], squares[kTileGroups];
+    const Place p = place_of(s, blockIdx.x);
+    const uint32_t row = thread_row(s, p, V);
+    const Rows rows = rows_at<D, V>(x, p, s.x_image, s.x_pixel, s);
+    Differences<V, Q> sums;
+    stream<D, V, kUnroll>(rows, s.rows, p.size, row, [&](uint32_t k, const PackedVector<D, V>& packed) {
+        float v[V];
+        unpack<D, V>(packed, v);
+        sums.add(v, k == 0);
+    });
     // the group's mean, then everybody's deviations from it
+    const uint32_t groups = groups_of_tile(s, p.tile), width = s.columns * Q, slots = s.per_group / W;
+    const uint32_t slot = threadIdx.x % s.columns * Q, at = threadIdx.x / s.columns * width + slot;
+    const bool in_block = threadIdx.x / s.columns < s.rows;
+    const uint32_t count = row < p.size ? (p.size - row + s.rows - 1) / s.rows : 0;
+    const float n = (float)(count * W), share = count ? 1.0f / n : 0.0f, in_group = (float)p.size * (float)s.per_group;
+    if (in_block)
 #pragma unroll
-    for (int j = 0; j < V; ++j) values[j] = count * mean[j];
-    group_sums<V, V>(column_sums<V>(values, s.columns, s.rows, lds), 0, s, group);
-    if (p.active) {
+        for (int q = 0; q < Q; ++q) lds[at + q] = sums.sum(q, n);
+    __syncthreads();
+    group_sums(lds, width, s.rows, slots, groups, group);
+    if (in_block)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float d = mean[j] - group[(p.channel + j) / s.per_group] / in_group;
-            values[j] = fmaf(count * d, d, m2[j]);
+        for (int q = 0; q < Q; ++q) {
+            // the slots of a last tile's missing groups are nobody's
+            const float of_group = (slot + q) / slots < groups ? group[(slot + q) / slots] / in_group : 0.0f;
+            lds[at + q] = sums.deviations(q, n, share, of_group);
         }
-    }
-    float* squares = group + s.groups;
-    group_sums<V, V>(column_sums<V>(values, s.columns, s.rows, lds), 0, s, squares);
-    for (uint32_t g = threadIdx.x; g < s.groups; g += kThreads)
-        partial[(size_t)blockIdx.x * s.groups + g] = make_float2(group[g] / in_group, squares[g]);
+    __syncthreads();
+    group_sums(lds, width, s.rows, slots, groups, squares);
+    if (threadIdx.x < groups)
+        partial[sums_at(s, p, threadIdx.x) + p.slab] = make_float2(group[threadIdx.x] / in_group, squares[threadIdx.x]);
 }
 
-__device__ __forceinline__ float slab_count(const Shape& s, uint32_t slab) {
-    return (float)(min((slab + 1) * s.slab_pixels, s.pixels) - slab * s.slab_pixels) * (float)s.per_group;
-}
-
-// The moments of one image's groups from its slabs': threads side by side take the groups, the others every so many slabs.
-__device__ __forceinline__ void fold_moments(const float2* partial, const Shape& s, float4* lds, float2* result) {
-    const uint32_t lanes = kThreads / s.groups, group = threadIdx.x % s.groups, lane = threadIdx.x / s.groups;
-    float n = 0.0f, mean = 0.0f, m2 = 0.0f;
-    if (lane < lanes)
+// A group's moments from its slabs', by a power of two of lanes, in all of them: a lane's slabs with the first one's mean as the
+// pivot, then the lanes' deviations from the mean of all. `mine` is null for lanes of no group.
+__device__ __forceinline__ float2 fold_moments(const float2* mine, const Shape& s, uint32_t lane, uint32_t lanes) {
+    const float count = (float)s.pixels * (float)s.per_group, of_slab = (float)s.slab_pixels * (float)s.per_group;
+    const float of_last = (float)(s.pixels - (s.slabs - 1) * s.slab_pixels) * (float)s.per_group;
+    float n = 0.0f, pivot = 0.0f, s1 = 0.0f, s2 = 0.0f;
+    if (mine && lane < s.slabs) {
+        pivot = mine[lane].x;
+#pragma unroll 8
         for (uint32_t slab = lane; slab < s.slabs; slab += lanes) {
-            const float2 b = partial[(size_t)slab * s.groups + group];
-            merge_moments(n, mean, m2, slab_count(s, slab), b.x, b.y);
-        }
-    lds[threadIdx.x] = make_float4(n, mean, m2, 0.0f);
-    uint32_t half = 1;
-    while (half < lanes) half <<= 1;
-    for (half >>= 1; half > 0; half >>= 1) {
-        __syncthreads();
-        if (lane < half && lane + half < lanes) {
-            float4 a = lds[threadIdx.x];
-            const float4 b = lds[threadIdx.x + half * s.groups];
-            merge_moments(a.x, a.y, a.z, b.x, b.y, b.z);
-            lds[threadIdx.x] = a;
+            const float2 v = mine[slab];
+            const float weight = slab + 1 < s.slabs ? of_slab : of_last, d = v.x - pivot;
+            n += weight;
+            s1 = fmaf(weight, d, s1);
+            s2 += fmaf(weight * d, d, v.y);
         }
     }
+    const float share = n > 0.0f ? s1 / n : 0.0f;
+    const float mean = lanes_sum(fmaf(n, pivot, s1), lanes) / count, d = pivot + share - mean;
+    const float squares = lanes_sum(fmaf(n * d, d, fmaf(-s1, share, s2)), lanes);
+    return make_float2(mean, 1.0f / sqrtf(fmaxf(squares, 0.0f) / count + s.eps));
+}
+
+// ... and the means A and B of the gradient pass
+__device__ __forceinline__ float2 fold_gradients(const float2* mine, const Shape& s, uint32_t lane, uint32_t lanes) {
+    float a = 0.0f, b = 0.0f;
+    if (mine)
+#pragma unroll 8
+        for (uint32_t slab = lane; slab < s.slabs; slab += lanes) {
+            a += mine[slab].x;
+            b += mine[slab].y;
+        }
+    const float count = (float)s.pixels * (float)s.per_group;
+    return make_float2(lanes_sum(a, lanes) / count, lanes_sum(b, lanes) / count);
+}
+
+// Of one tile of an image, into LDS: by every block of the launch that needs them where they are few ...
+template <typename F>
+__device__ __forceinline__ void fold_tile(const float2* partial, const Shape& s, const Place& p, float2* folded, F fold) {
+    const uint32_t groups = groups_of_tile(s, p.tile), lanes = lanes_for(groups), lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+    const float2 m = fold(group < groups ? partial + sums_at(s, p, group) : nullptr, s, lane, lanes);
+    if (lane == 0 && group < groups) folded[group] = m;
     __syncthreads();
-    if (threadIdx.x < s.groups) {
-        const float4 a = lds[threadIdx.x];
-        result[threadIdx.x] = make_float2(a.y, 1.0f / sqrtf(a.z / a.x + s.eps));
-    }
-    __syncthreads();
 }
 
-// The same for maps of many groups, a wave per (image, group)
-__global__ void __launch_bounds__(kThreads) k_combine_moments(const float2* __restrict__ partial, float2* __restrict__ moments,
-                                                              Shape s) {
-    const uint32_t item = blockIdx.x * (kThreads / 64) + threadIdx.x / 64u, image = item / s.groups, group = item % s.groups;
-    if (image >= s.n) return;
-    float n = 0.0f, mean = 0.0f, m2 = 0.0f;
-    for (uint32_t slab = lane_id(); slab < s.slabs; slab += 64) {
-        const float2 b = partial[((size_t)image * s.slabs + slab) * s.groups + group];
-        merge_moments(n, mean, m2, slab_count(s, slab), b.x, b.y);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float nb = __shfl_xor(n, o, 64), mean_b = __shfl_xor(mean, o, 64), m2_b = __shfl_xor(m2, o, 64);
-        merge_moments(n, mean, m2, nb, mean_b, m2_b);
-    }
-    if (lane_id() == 0) moments[item] = make_float2(mean, 1.0f / sqrtf(m2 / n + s.eps));
+// ... else in a launch of its own, a wave per (image, group)
+__device__ __forceinline__ const float2* sums_of_wave(const float2* partial, const Shape& s, uint32_t item) {
+    const uint32_t image = item / s.groups, group = item % s.groups;
+    if (image >= s.n) return nullptr;
+    return partial + ((size_t)(image * s.tiles + group / s.tile_groups) * s.tile_groups + group % s.tile_groups) * s.slabs;
 }
 
-template <int V>
-__device__ __forceinline__ Moments<V> channel_moments(const float2* of_image, const Shape& s, uint32_t channel) {
-    Moments<V> m;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float2 v = of_image[(channel + j) / s.per_group];
-        m.mean[j] = v.x;
-        m.rstd[j] = v.y;
-    }
-    return m;
+__global__ void __launch_bounds__(kThreads) k_combine_moments(const float2* __restrict__ partial, float2* __restrict__ moments, Shape s) {
+    const uint32_t item = blockIdx.x * (kThreads / 64) + threadIdx.x / 64u;
+    const float2* mine = sums_of_wave(partial, s, item);
+    const float2 m = fold_moments(mine, s, lane_id(), 64);
+    if (mine && lane_id() == 0) moments[item] = m;
 }
 
-// `partial` is null where k_combine_moments has run; else the first block of each image also writes its moments.
-template <int D, int V>
+// The first `parameter_blocks` blocks add up dweight and dbias.
+__global__ void __launch_bounds__(kThreads) k_combine_gradients(const float2* __restrict__ of_groups, const float2* __restrict__ of_channels,
+                                                                float2* __restrict__ means, void* __restrict__ dweight,
+                                                                void* __restrict__ dbias, uint32_t parameter_blocks, Shape s) {
+    __shared__ float lds[column_floats<2>(kThreads)];
+    if (blockIdx.x < parameter_blocks) {
+        add_parameter_gradients(of_channels, s.n * s.slabs, dweight, dbias, s, blockIdx.x, lds);
+        return;
+    }
+    const uint32_t item = (blockIdx.x - parameter_blocks) * (kThreads / 64) + threadIdx.x / 64u;
+    const float2* mine = sums_of_wave(of_groups, s, item);
+    const float2 m = fold_gradients(mine, s, lane_id(), 64);
+    if (mine && lane_id() == 0) means[item] = m;
+}
+
+// `partial` is null where k_combine_moments has run; else the first block of each tile of an image also writes its moments.
+template <int D, int V, int Q>
 __global__ void __launch_bounds__(kThreads) k_apply(const void* __restrict__ x, const float2* __restrict__ partial,
                                                     const void* __restrict__ weight, const void* __restrict__ bias,
                                                     void* __restrict__ y, float2* __restrict__ moments, Shape s, Dropout d) {
-    __shared__ float4 lds[kThreads];
-    __shared__ float2 folded[kThreads];
-    const Place p = place_of<V>(s, blockIdx.x);
-    float2* global = moments + (size_t)p.image * s.groups;
+    __shared__ float2 folded[kTileGroups];
+    const Place p = place_of(s, blockIdx.x);
+    float2* of_tile = moments + (size_t)p.image * s.groups + p.tile * s.tile_groups;
+    const float2* m = of_tile;
     if (partial) {
-        fold_moments(partial + (size_t)p.image * s.slabs * s.groups, s, lds, folded);
-        if (p.slab == 0 && threadIdx.x < s.groups) global[threadIdx.x] = folded[threadIdx.x];
+        fold_tile(partial, s, p, folded, fold_moments);
+        if (p.slab == 0 && threadIdx.x < groups_of_tile(s, p.tile)) of_tile[threadIdx.x] = folded[threadIdx.x];
+        m = folded;
     }
-    if (!p.active) return;
-    const Moments<V> m = partial ? channel_moments<V>(folded, s, p.channel) : channel_moments<V>(global, s, p.channel);
-    const Parameters<V> c = load_parameters<V>(s, weight, bias, p.channel);
+    const uint32_t row = thread_row(s, p, V);
+    if (row >= p.size) return;
+    const Affine<V, Q> a = load_affine<V, Q>(s, m, p.channel, p.channel + threadIdx.x % s.columns * V, weight, bias);
     const uint64_t seed = dropout_seed(d);
-    const size_t base = (size_t)p.image * s.x_image + p.channel;
-    const size_t out = (size_t)p.image * s.pixels * s.channels + p.channel;
-    uint32_t r = p.begin + p.row;
-    for (; r + (kUnroll - 1) * s.rows < p.end; r += kUnroll * s.rows) {
-        PackedVector<D, V> packed[kUnroll];
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k) packed[k] = load_packed<D, V>(x, base + (size_t)(r + k * s.rows) * s.x_pixel);
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k)
-            apply_vector<D, V, V>(s, d, seed, m, c, packed[k], y, out + (size_t)(r + k * s.rows) * s.channels);
-    }
-    for (; r < p.end; r += s.rows)
-        apply_vector<D, V, V>(s, d, seed, m, c, load_packed<D, V>(x, base + (size_t)r * s.x_pixel), y, out + (size_t)r * s.channels);
+    const Rows ry = rows_at<D, V>(y, p, (uint64_t)s.pixels * s.channels, s.channels, s);
+    const Numbers numbers = numbers_at<V>(p, s);
+    stream<D, V, kUnroll>(rows_at<D, V>(x, p, s.x_image, s.x_pixel, s), s.rows, p.size, row, [&](uint32_t k, const PackedVector<D, V>& packed) {
+        apply_vector<D, V, Q>(s, d, seed, a, packed, ry, numbers, k);
+    });
 }
 
 // {sum dz, sum dz * xhat} of every (image, slab, channel), and both weighted and summed of every (image, slab, group)
-template <int D, int V>
+template <int D, int V, int Q>
 __global__ void __launch_bounds__(kThreads) k_gradient_sums(const void* __restrict__ x, const void* __restrict__ dy,
-                                                            const float2* __restrict__ moments, const void* __restrict__ weight,
+                                                            const float2* __restrict__ all_moments, const void* __restrict__ weight,
                                                             const void* __restrict__ bias, float2* __restrict__ of_channels,
                                                             float2* __restrict__ of_groups, Shape s, Dropout d) {
-    INPC_DYNAMIC_LDS(float, lds);   // column_sums of 2 V values per thread, then two floats per group
-    float *group_a = lds + (kThreads + 32) * 2 * V, *group_b = group_a + s.groups;
-    const Place p = place_of<V>(s, blockIdx.x);
+    __shared__ float lds[column_floats<2 * V>(kThreads)];
+    const Place p = place_of(s, blockIdx.x);
+    const uint32_t row = thread_row(s, p, V);
+    const float2* moments = all_moments + (size_t)p.image * s.groups;
     float total[2 * V];
 #pragma unroll
     for (int j = 0; j < 2 * V; ++j) total[j] = 0.0f;
-    Parameters<V> c;
-    if (p.active) {
-        const Moments<V> m = channel_moments<V>(moments + (size_t)p.image * s.groups, s, p.channel);
-        c = load_parameters<V>(s, weight, bias, p.channel);
+    if (row < p.size) {
+        const Affine<V, Q> a = load_affine<V, Q>(s, moments, 0, p.channel + threadIdx.x % s.columns * V, weight, bias);
         const uint64_t seed = dropout_seed(d);
-        const size_t base = (size_t)p.image * s.x_image + p.channel, gbase = (size_t)p.image * s.g_image + p.channel;
-        const size_t out = (size_t)p.image * s.pixels * s.channels + p.channel;
-        const auto add = [&](uint32_t r, const PackedVector<D, V>& px, const PackedVector<D, V>& pg) {
-            float v[V], g[V];
-            gradient_vector<D, V, V>(s, d, seed, m, c, px, pg, out + (size_t)r * s.channels, v, g);
+        const Numbers numbers = numbers_at<V>(p, s);
+        stream<D, V, kUnrollBackward>(rows_at<D, V>(x, p, s.x_image, s.x_pixel, s), rows_at<D, V>(dy, p, s.g_image, s.g_pixel, s), s.rows, p.size, row,
+                                      [&](uint32_t k, const PackedVector<D, V>& px, const PackedVector<D, V>& pg) {
+                                          float v[V], g[V];
+                                          gradient_vector<D, V, Q>(s, d, seed, a, px, pg, number_of(numbers, k), v, g);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                total[j] += g[j];
-                total[V + j] = fmaf(g[j], v[j], total[V + j]);
-            }
-        };
-        uint32_t r = p.begin + p.row;
-        for (; r + (kUnroll - 1) * s.rows < p.end; r += kUnroll * s.rows) {
-            PackedVector<D, V> px[kUnroll], pg[kUnroll];
-#pragma unroll
-            for (int k = 0; k < kUnroll; ++k) {
-                px[k] = load_packed<D, V>(x, base + (size_t)(r + k * s.rows) * s.x_pixel);
-                pg[k] = load_packed<D, V>(dy, gbase + (size_t)(r + k * s.rows) * s.g_pixel);
-            }
-#pragma unroll
-            for (int k = 0; k < kUnroll; ++k) add(r + k * s.rows, px[k], pg[k]);
-        }
-        for (; r < p.end; r += s.rows)
-            add(r, load_packed<D, V>(x, base + (size_t)r * s.x_pixel), load_packed<D, V>(dy, gbase + (size_t)r * s.g_pixel));
+                                          for (int j = 0; j < V; ++j) {
+                                              total[j] += g[j];
+                                              total[V + j] = fmaf(g[j], v[j], total[V + j]);
+                                          }
+                                      });
     }
-    float* totals = (float*)column_sums<2 * V>(total, s.columns, s.rows, lds);
-    for (uint32_t i = threadIdx.x; i < s.channels; i += kThreads) {
-        float *sum = totals + i / V * (2 * V) + i % V, *product = sum + V;
-        of_channels[(size_t)blockIdx.x * s.channels + i] = make_float2(*sum, *product);
-        const float w = weight ? load_element(weight, s.param_dtype, i) : 1.0f;
-        *sum *= w;
-        *product *= w;
+    const uint32_t groups = groups_of_tile(s, p.tile), first = p.tile * s.tile_groups, channels = groups * s.per_group;
+    float2* mine = of_channels + ((size_t)p.image * s.slabs + p.slab) * s.channels + p.channel;
+    float* totals = column_sums<2 * V>(total, s.columns, s.rows, lds);
+    // a channel's two sums, and weighted in place
+    for (uint32_t i = threadIdx.x; i < channels; i += kThreads) {
+        float* of_channel = totals + i / V * (2 * V) + i % V;
+        const float2 sum = make_float2(of_channel[0], of_channel[V] * moments[first + i / s.per_group].y);
+        const float w = weight ? load_element(weight, s.param_dtype, p.channel + i) : 1.0f;
+        mine[i] = sum;
+        of_channel[0] = sum.x * w;
+        of_channel[V] = sum.y * w;
     }
     __syncthreads();
-    group_sums<V, 2 * V>(totals, 0, s, group_a);
-    group_sums<V, 2 * V>(totals, 1, s, group_b);
-    for (uint32_t g = threadIdx.x; g < s.groups; g += kThreads)
-        of_groups[(size_t)blockIdx.x * s.groups + g] = make_float2(group_a[g], group_b[g]);
-}
-
-// The means A and B of one image's groups from its slabs' sums, as fold_moments
-__device__ __forceinline__ void fold_gradients(const float2* partial, const Shape& s, float2* lds, float2* result) {
-    const uint32_t lanes = kThreads / s.groups, group = threadIdx.x % s.groups, lane = threadIdx.x / s.groups;
-    float2 t = make_float2(0.0f, 0.0f);
-    if (lane < lanes)
-        for (uint32_t slab = lane; slab < s.slabs; slab += lanes) {
-            const float2 b = partial[(size_t)slab * s.groups + group];
-            t.x += b.x;
-            t.y += b.y;
-        }
-    lds[threadIdx.x] = t;
-    uint32_t half = 1;
-    while (half < lanes) half <<= 1;
-    for (half >>= 1; half > 0; half >>= 1) {
-        __syncthreads();
-        if (lane < half && lane + half < lanes) {
-            lds[threadIdx.x].x += lds[threadIdx.x + half * s.groups].x;
-            lds[threadIdx.x].y += lds[threadIdx.x + half * s.groups].y;
-        }
-    }
-    __syncthreads();
-    if (threadIdx.x < s.groups) {
-        const float count = (float)s.pixels * (float)s.per_group;
-        result[threadIdx.x] = make_float2(lds[threadIdx.x].x / count, lds[threadIdx.x].y / count);
-    }
-    __syncthreads();
-}
-
-__global__ void __launch_bounds__(kThreads) k_combine_gradients(const float2* __restrict__ partial, float2* __restrict__ means,
-                                                                Shape s) {
-    const uint32_t item = blockIdx.x * (kThreads / 64) + threadIdx.x / 64u, image = item / s.groups, group = item % s.groups;
-    if (image >= s.n) return;
+    const uint32_t lanes = lanes_for(groups), lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
     float a = 0.0f, b = 0.0f;
-    for (uint32_t slab = lane_id(); slab < s.slabs; slab += 64) {
-        const float2 v = partial[((size_t)image * s.slabs + slab) * s.groups + group];
-        a += v.x;
-        b += v.y;
-    }
-    a = wave_sum(a);
-    b = wave_sum(b);
-    const float count = (float)s.pixels * (float)s.per_group;
-    if (lane_id() == 0) means[item] = make_float2(a / count, b / count);
+    if (group < groups)
+        for (uint32_t i = group * s.per_group + lane; i < (group + 1) * s.per_group; i += lanes) {
+            const float* of_channel = totals + i / V * (2 * V) + i % V;
+            a += of_channel[0];
+            b += of_channel[V];
+        }
+    a = lanes_sum(a, lanes);
+    b = lanes_sum(b, lanes);
+    if (lane == 0 && group < groups) of_groups[sums_at(s, p, group) + p.slab] = make_float2(a, b);
 }
 
-// The first `parameter_blocks` blocks add up dweight and dbias, the others write dx. `means` where k_combine_gradients has run,
-// else null.
-template <int D, int V>
+// `means` is null where k_combine_gradients has not run: then the first `parameter_blocks` blocks add up dweight and dbias.
+template <int D, int V, int Q>
 __global__ void __launch_bounds__(kThreads) k_input_gradient(const void* __restrict__ x, const void* __restrict__ dy,
                                                              const float2* __restrict__ moments, const float2* __restrict__ of_channels,
                                                              const float2* __restrict__ of_groups, const float2* __restrict__ means,
                                                              const void* __restrict__ weight, const void* __restrict__ bias,
                                                              void* __restrict__ dx, void* __restrict__ dweight,
                                                              void* __restrict__ dbias, uint32_t parameter_blocks, Shape s, Dropout d) {
-    __shared__ float lds[kThreads * 2 + 64];
-    __shared__ float2 folded[kThreads];
+    __shared__ float lds[column_floats<2>(kThreads)];
+    __shared__ float2 folded[kTileGroups];
     if (blockIdx.x < parameter_blocks) {
-        add_parameter_gradients(of_channels, (size_t)s.n * s.slabs, dweight, dbias, s, blockIdx.x, lds);
+        add_parameter_gradients(of_channels, s.n * s.slabs, dweight, dbias, s, blockIdx.x, lds);
         return;
     }
-    const Place p = place_of<V>(s, blockIdx.x - parameter_blocks);
-    const float2* ab = means + (size_t)p.image * s.groups;
+    const Place p = place_of(s, blockIdx.x - parameter_blocks);
+    const float2* ab = means + (size_t)p.image * s.groups + p.tile * s.tile_groups;
     if (!means) {
-        fold_gradients(of_groups + (size_t)p.image * s.slabs * s.groups, s, (float2*)lds, folded);
+        fold_tile(of_groups, s, p, folded, fold_gradients);
         ab = folded;
     }
-    if (!p.active) return;
-    const Moments<V> m = channel_moments<V>(moments + (size_t)p.image * s.groups, s, p.channel);
-    const Parameters<V> c = load_parameters<V>(s, weight, bias, p.channel);
-    float mean_a[V], mean_b[V];
+    const uint32_t row = thread_row(s, p, V), channel = p.channel + threadIdx.x % s.columns * V;
+    if (row >= p.size) return;
+    const Affine<V, Q> a = load_affine<V, Q>(s, moments + (size_t)p.image * s.groups, 0, channel, weight, bias);
+    float k1[Q], k2[Q];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float2 v = ab[(p.channel + j) / s.per_group];
-        mean_a[j] = v.x;
-        mean_b[j] = v.y;
+    for (int q = 0; q < Q; ++q) {
+        const float2 v = ab[(channel - p.channel + q * (V / Q)) / s.per_group];
+        k1[q] = v.x * a.rstd[q];
+        k2[q] = v.y * a.rstd[q] * a.rstd[q];
     }
     const uint64_t seed = dropout_seed(d);
-    const size_t base = (size_t)p.image * s.x_image + p.channel, gbase = (size_t)p.image * s.g_image + p.channel;
-    const size_t out = (size_t)p.image * s.pixels * s.channels + p.channel;
-    uint32_t r = p.begin + p.row;
-    for (; r + (kUnroll - 1) * s.rows < p.end; r += kUnroll * s.rows) {
-        PackedVector<D, V> px[kUnroll], pg[kUnroll];
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            px[k] = load_packed<D, V>(x, base + (size_t)(r + k * s.rows) * s.x_pixel);
-            pg[k] = load_packed<D, V>(dy, gbase + (size_t)(r + k * s.rows) * s.g_pixel);
-        }
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k)
-            input_gradient_vector<D, V, V>(s, d, seed, m, mean_a, mean_b, c, px[k], pg[k], dx,
-                                           out + (size_t)(r + k * s.rows) * s.channels);
-    }
-    for (; r < p.end; r += s.rows)
-        input_gradient_vector<D, V, V>(s, d, seed, m, mean_a, mean_b, c, load_packed<D, V>(x, base + (size_t)r * s.x_pixel),
-                                       load_packed<D, V>(dy, gbase + (size_t)r * s.g_pixel), dx, out + (size_t)r * s.channels);
+    const Rows rdx = rows_at<D, V>(dx, p, (uint64_t)s.pixels * s.channels, s.channels, s);
+    const Numbers numbers = numbers_at<V>(p, s);
+    stream<D, V, kUnrollBackward>(rows_at<D, V>(x, p, s.x_image, s.x_pixel, s), rows_at<D, V>(dy, p, s.g_image, s.g_pixel, s), s.rows, p.size, row,
+                                  [&](uint32_t k, const PackedVector<D, V>& px, const PackedVector<D, V>& pg) {
+                                      input_gradient_vector<D, V, Q>(s, d, seed, a, k1, k2, px, pg, rdx, numbers, k);
+                                  });
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
@@ -786,49 +773,64 @@ inline Shape base_shape(const inpc_group_norm_config& cfg) {
 }
 
 // Bytes of one group of one image up to which the single form runs.
-constexpr uint64_t kSingleBytes = 128 * 1024;
+constexpr uint64_t kSingleBytes = 32 * 1024;
+
+// Groups of a tile of the split form with vectors of v elements: as many as fit, with boundaries on vectors' boundaries; 0 where
+// not even the fewest do.
+inline uint32_t tile_groups_of(const inpc_group_norm_config& cfg, int v) {
+    const uint32_t per_group = cfg.channels / cfg.groups;
+    uint32_t unit = 1;   // groups whose channels are whole vectors
+    while ((uint64_t)unit * per_group % (uint32_t)v != 0) unit *= 2;
+    const uint64_t fit = std::min<uint64_t>((uint64_t)kThreads * v / per_group, kTileGroups);
+    return (uint32_t)std::min<uint64_t>(cfg.groups, fit / unit * unit);
+}
 
 inline bool runs_single(const inpc_group_norm_config& cfg, int v) {
     const uint64_t bytes = (uint64_t)cfg.n_pixels * (cfg.channels / cfg.groups) * element_bytes(cfg.dtype);
-    return bytes <= kSingleBytes || cfg.channels / (uint32_t)v > (uint32_t)kThreads || cfg.groups > (uint32_t)kThreads;
+    return bytes <= kSingleBytes || tile_groups_of(cfg, v) == 0;
 }
 
 // Threads of a block of the single form: as many as the group has vectors, in whole waves.
-inline Shape single_shape(const inpc_group_norm_config& cfg, int v, int most, uint32_t& threads) {
+inline Shape single_shape(const inpc_group_norm_config& cfg, int v, uint32_t& threads) {
     Shape s = base_shape(cfg);
     const uint64_t vectors = (uint64_t)s.per_group / (uint32_t)v, all = vectors * s.pixels;
     threads = 64;
-    while (threads < (uint32_t)most && threads < all) threads *= 2;
+    while (threads < (uint32_t)kMaxThreads && threads < all) threads *= 2;
     s.columns = (uint32_t)std::min<uint64_t>(vectors, threads);
     s.rows = threads / s.columns;
     return s;
 }
 
-inline Shape split_shape(const inpc_group_norm_config& cfg, int v) {
+inline Shape split_shape(const inpc_group_norm_config& cfg, int v, uint32_t blocks = kSumBlocks) {
     Shape s = base_shape(cfg);
-    s.columns = cfg.channels / (uint32_t)v;
+    s.tile_groups = tile_groups_of(cfg, v);
+    s.tiles = div_up(s.groups, s.tile_groups);
+    s.columns = s.tile_groups * s.per_group / (uint32_t)v;
     s.rows = kThreads / s.columns;
-    const uint64_t per_image = std::max<uint64_t>(1, kFillBlocks / s.n), step = (uint64_t)s.rows * kUnroll;
-    const uint64_t wanted = (s.pixels + per_image - 1) / per_image;
+    const uint64_t runs = (uint64_t)s.n * s.tiles, per_run = std::max<uint64_t>(1, blocks / runs);
+    const uint64_t wanted = (s.pixels + per_run - 1) / per_run;
+    const uint32_t step = s.rows * kUnroll;
     s.slab_pixels = (uint32_t)((wanted + step - 1) / step * step);
     s.slabs = div_up(s.pixels, s.slab_pixels);
     return s;
 }
 
-// What a call may need, whatever its alignment: [sums per (image, channel)] or [sums per (image, slab, group)] [sums per
-// (image, slab, channel)] [means per (image, group)]
+inline bool folds(const Shape& s) { return (uint64_t)s.slabs * s.tile_groups <= kFoldedSums; }
+
+// What a call may need: [sums per (image, tile, group of a tile, slab)] [backward: sums per (image, slab, channel)] [means per
+// (image, group)], the second with one slab in the single form.
 struct Workspace {
     size_t of_groups, of_channels, means, bytes;
 };
 inline Workspace split_workspace(const Shape& s, bool backward) {
     Workspace w;
-    const size_t slabs = (size_t)s.n * s.slabs;
     w.of_groups = 0;
-    w.of_channels = align_up(slabs * s.groups * sizeof(float2), 256);
-    w.means = w.of_channels + (backward ? align_up(slabs * s.channels * sizeof(float2), 256) : 0);
-    w.bytes = w.means + (backward ? align_up((size_t)s.n * s.groups * sizeof(float2), 256) : 0);
+    w.of_channels = align_up((size_t)s.n * s.tiles * s.tile_groups * s.slabs * sizeof(float2), 256);
+    w.means = w.of_channels + (backward ? align_up((size_t)s.n * s.slabs * s.channels * sizeof(float2), 256) : 0);
+    w.bytes = w.means + (backward ? (size_t)s.n * s.groups * sizeof(float2) : 0);
     return w;
 }
+// ... whatever the alignment of its tensors
 inline size_t workspace_bytes(const inpc_group_norm_config& cfg, bool backward) {
     size_t most = backward && cfg.n_images > 1 ? (size_t)cfg.n_images * cfg.channels * sizeof(float2) : 0;
     for (int v = (int)(16 / element_bytes(cfg.dtype)); v >= 1; v /= 2)
@@ -848,8 +850,11 @@ inline int check_config(const inpc_group_norm_config* cfg, const char* what) {
     if (cfg->channels > INPC_GROUP_NORM_MAX_CHANNELS || cfg->n_pixels >= (1u << 30))
         return fail(INPC_E_UNSUPPORTED, "%s: at most %u channels and fewer than 2^30 pixels per image", what,
                     INPC_GROUP_NORM_MAX_CHANNELS);
+    // a thread's offset in a block's rows is counted in 32 bits
+    if (cfg->input_pixel_stride >= (1u << 19) || cfg->grad_pixel_stride >= (1u << 19))
+        return fail(INPC_E_UNSUPPORTED, "%s: pixel strides are below 2^19 elements", what);
     // blocks are counted in 31 bits
-    if ((uint64_t)cfg->n_images * cfg->groups > 0x7FFFFFFFu || (uint64_t)cfg->n_images + kFillBlocks > 0x7FFFFFFFu)
+    if ((uint64_t)cfg->n_images * cfg->groups > 0x7FFFFFFFu || (uint64_t)cfg->n_images + kApplyBlocks > 0x7FFFFFFFu)
         return fail(INPC_E_UNSUPPORTED, "%s: too many images", what);
     if (!(cfg->eps >= 0.0f)) return fail(INPC_E_INVALID_ARGUMENT, "%s: eps must not be negative", what);
     if (!valid_probability(cfg->dropout_p)) return fail(INPC_E_INVALID_ARGUMENT, "%s: the dropout probability is outside [0, 1]", what);
@@ -877,7 +882,7 @@ template <int D, int V>
 int forward_single(const inpc_group_norm_config& cfg, const void* x, const void* weight, const void* bias, void* y, float2* moments,
                    hipStream_t stream) {
     uint32_t threads = 0;
-    const Shape s = single_shape(cfg, V, kMaxThreads, threads);
+    const Shape s = single_shape(cfg, V, threads);
     const Dropout d = make_dropout(cfg.dropout_p, cfg.seed, cfg.seed_dev, cfg.offset);
     INPC_LAUNCH("group_norm_single", (k_single<D, V>), dim3(s.n * s.groups), dim3(threads), stream, x, weight, bias, y, moments, s, d);
     return INPC_OK;
@@ -887,33 +892,50 @@ template <int D, int V>
 int backward_single(const inpc_group_norm_config& cfg, const void* x, const void* dy, const float2* moments, const void* weight,
                     const void* bias, void* dx, void* dweight, void* dbias, char* ws, hipStream_t stream) {
     uint32_t threads = 0;
-    const Shape s = single_shape(cfg, V, kMaxThreadsBackward, threads);
+    const Shape s = single_shape(cfg, V, threads);
     const Dropout d = make_dropout(cfg.dropout_p, cfg.seed, cfg.seed_dev, cfg.offset);
     const bool later = s.n > 1 && (dweight || dbias);
     float2* sums = later ? (float2*)ws : nullptr;
     INPC_NORM_LAUNCH_LDS("group_norm_single_backward", (k_single_backward<D, V>), dim3(s.n * s.groups), dim3(threads),
-                         (size_t)(threads + 32) * 2 * V * sizeof(float), stream, x, dy, moments, weight, bias, dx,
+                         column_floats<2 * V>(threads) * sizeof(float), stream, x, dy, moments, weight, bias, dx,
                          later ? (void*)nullptr : dweight, later ? (void*)nullptr : dbias, sums, s, d);
     if (later)
         INPC_LAUNCH("group_norm_parameter_gradients", k_parameter_gradients, dim3(div_up(s.channels, kParameterColumns)),
-                    dim3(kThreads), stream, sums, dweight, dbias, s);
+                    dim3(kThreads), stream, sums, s.n, dweight, dbias, s);
     return INPC_OK;
 }
+
+// k<D, V, Q> with the slots that vectors of V channels fall into
+#define INPC_NORM_SLOTS(k, per_group, ...)                                             \
+    do {                                                                               \
+        if ((per_group) % V == 0) {                                                    \
+            __VA_ARGS__((k<D, V, 1>))                                                  \
+        } else if (V > 2 && (per_group) * 2 == V) {                                    \
+            __VA_ARGS__((k<D, V, V < 4 ? V : 2>))                                      \
+        } else {                                                                       \
+            __VA_ARGS__((k<D, V, V>))                                                  \
+        }                                                                              \
+    } while (0)
 
 template <int D, int V>
 int forward_split(const inpc_group_norm_config& cfg, const void* x, const void* weight, const void* bias, void* y, float2* moments,
                   char* ws, hipStream_t stream) {
     const Shape s = split_shape(cfg, V);
     const Dropout d = make_dropout(cfg.dropout_p, cfg.seed, cfg.seed_dev, cfg.offset);
-    const bool fold = (uint64_t)s.slabs * s.groups <= kFoldedSums;
     float2* partial = (float2*)(ws + split_workspace(s, false).of_groups);
-    INPC_NORM_LAUNCH_LDS("group_norm_moments", (k_moments<D, V>), dim3(s.n * s.slabs), dim3(kThreads),
-                         ((size_t)(kThreads + 32) * V + 2 * s.groups) * sizeof(float), stream, x, partial, s);
+#define INPC_NORM_MOMENTS(k) INPC_LAUNCH("group_norm_moments", k, dim3(s.n * s.tiles * s.slabs), dim3(kThreads), stream, x, partial, s);
+    INPC_NORM_SLOTS(k_moments, s.per_group, INPC_NORM_MOMENTS);
+#undef INPC_NORM_MOMENTS
+    const bool fold = folds(s);
     if (!fold)
-        INPC_LAUNCH("group_norm_combine_moments", k_combine_moments, dim3(div_up(s.n * s.groups, kThreads / 64)), dim3(kThreads),
-                    stream, partial, moments, s);
-    INPC_LAUNCH("group_norm_apply", (k_apply<D, V>), dim3(s.n * s.slabs), dim3(kThreads), stream, x,
-                fold ? (const float2*)partial : (const float2*)nullptr, weight, bias, y, moments, s, d);
+        INPC_LAUNCH("group_norm_combine_moments", k_combine_moments, dim3(div_up(s.n * s.groups, kThreads / 64)), dim3(kThreads), stream,
+                    partial, moments, s);
+    const Shape a = fold ? s : split_shape(cfg, V, kApplyBlocks);
+    const float2* to_fold = fold ? partial : nullptr;
+#define INPC_NORM_APPLY(k)                                                                                                              \
+    INPC_LAUNCH("group_norm_apply", k, dim3(a.n * a.tiles * a.slabs), dim3(kThreads), stream, x, to_fold, weight, bias, y, moments, a, d);
+    INPC_NORM_SLOTS(k_apply, s.per_group, INPC_NORM_APPLY);
+#undef INPC_NORM_APPLY
     return INPC_OK;
 }
 
@@ -923,18 +945,28 @@ int backward_split(const inpc_group_norm_config& cfg, const void* x, const void*
     const Shape s = split_shape(cfg, V);
     const Dropout d = make_dropout(cfg.dropout_p, cfg.seed, cfg.seed_dev, cfg.offset);
     const Workspace w = split_workspace(s, true);
-    const bool fold = (uint64_t)s.slabs * s.groups <= kFoldedSums;
     float2 *of_groups = (float2*)(ws + w.of_groups), *of_channels = (float2*)(ws + w.of_channels), *means = (float2*)(ws + w.means);
-    INPC_NORM_LAUNCH_LDS("group_norm_gradient_sums", (k_gradient_sums<D, V>), dim3(s.n * s.slabs), dim3(kThreads),
-                         ((size_t)(kThreads + 32) * 2 * V + 2 * s.groups) * sizeof(float), stream, x, dy, moments, weight, bias,
-                         of_channels, of_groups, s, d);
-    if (dx && !fold)
-        INPC_LAUNCH("group_norm_combine_gradients", k_combine_gradients, dim3(div_up(s.n * s.groups, kThreads / 64)), dim3(kThreads),
-                    stream, of_groups, means, s);
+#define INPC_NORM_SUMS(k)                                                                                                           \
+    INPC_LAUNCH("group_norm_gradient_sums", k, dim3(s.n * s.tiles * s.slabs), dim3(kThreads), stream, x, dy, moments, weight, bias,  \
+                of_channels, of_groups, s, d);
+    INPC_NORM_SLOTS(k_gradient_sums, s.per_group, INPC_NORM_SUMS);
+#undef INPC_NORM_SUMS
+    // dweight and dbias are added up next to whatever comes next
+    const bool fold = folds(s) && dx;
     const uint32_t parameter_blocks = dweight || dbias ? div_up(s.channels, kParameterColumns) : 0;
-    INPC_LAUNCH("group_norm_input_gradient", (k_input_gradient<D, V>), dim3(parameter_blocks + (dx ? s.n * s.slabs : 0)),
-                dim3(kThreads), stream, x, dy, moments, of_channels, of_groups, fold ? (const float2*)nullptr : (const float2*)means,
-                weight, bias, dx, dweight, dbias, parameter_blocks, s, d);
+    if (!fold)
+        INPC_LAUNCH("group_norm_combine_gradients", k_combine_gradients,
+                    dim3(parameter_blocks + (dx ? div_up(s.n * s.groups, kThreads / 64) : 0)), dim3(kThreads), stream, of_groups,
+                    of_channels, means, dweight, dbias, parameter_blocks, s);
+    if (!dx) return INPC_OK;
+    const Shape a = fold ? s : split_shape(cfg, V, kApplyBlocks);
+    const uint32_t first_blocks = fold ? parameter_blocks : 0;
+    const float2* combined = fold ? nullptr : means;
+#define INPC_NORM_GRADIENT(k)                                                                                                       \
+    INPC_LAUNCH("group_norm_input_gradient", k, dim3(first_blocks + a.n * a.tiles * a.slabs), dim3(kThreads), stream, x, dy, moments, \
+                of_channels, of_groups, combined, weight, bias, dx, dweight, dbias, first_blocks, a, d);
+    INPC_NORM_SLOTS(k_input_gradient, s.per_group, INPC_NORM_GRADIENT);
+#undef INPC_NORM_GRADIENT
     return INPC_OK;
 }
 

@@ -132,7 +132,7 @@ def _pixel_strides(t: torch.Tensor) -> tuple[int, int] | None:
     else:
         pixel = s_h if h != 1 else c
     image = s_n if n != 1 else h * w * pixel
-    if pixel < c or image < h * w * pixel:   # overlapping or expanded
+    if pixel < c or image < h * w * pixel or pixel >= 2**19:   # overlapping, expanded, or beyond the kernels' offsets
         return None
     return image, pixel
 
