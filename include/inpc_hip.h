@@ -579,7 +579,7 @@ int inpc_cauchy_loss_backward(const float* grad, const float* input, const float
 #define INPC_ACTIVATION_GELU 3 /* z (1 + erf(z / sqrt 2)) / 2                               */
 
 /* Group norm over channels-last feature maps: n_images images of n_pixels pixels of `channels` adjacent
- * values, the channels split into `groups` equal groups. Strides are in elements: from image to image and
+ * values, the channels split into `groups` equal groups, at most 8,388,607 groups of all images together. Strides are in elements: from image to image and
  * from pixel to pixel of the input (a slice of the channels of a wider map is an input like any other) and
  * of the output's gradient (backward only); pixel strides are below 2^19; output and input gradient are dense. */
 #define INPC_GROUP_NORM_MAX_CHANNELS 65536u

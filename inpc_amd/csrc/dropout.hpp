@@ -2,51 +2,53 @@
 // gradient, with the mask computed again (elements.hpp) instead of stored.
 #pragma once
 
+#include <algorithm>
+
 #include "elements.hpp"
 
 namespace inpc {
 namespace dropout {
 
 constexpr int kBlock = 256;
+constexpr uint64_t kMostBlocks = 1u << 20;   // a launch has fewer than 2^32 threads: beyond 2^31 values a thread takes several vectors
 
 // A thread takes eight consecutive elements, one draw of the generator. WIDE: both pointers are 16-byte aligned.
 template <int D, bool WIDE>
 __global__ void __launch_bounds__(kBlock) k_dropout(const void* __restrict__ x, void* __restrict__ y, uint64_t count, Dropout d) {
-    const uint64_t first = ((uint64_t)blockIdx.x * kBlock + threadIdx.x) * 8u;
-    if (first >= count) return;
-    const uint64_t seed = dropout_seed(d);
+    const uint64_t seed = dropout_seed(d), stride = (uint64_t)gridDim.x * kBlock * 8u;
     constexpr int W = D == INPC_DTYPE_F32 ? 4 : 8;
-    float v[8];
-    if (WIDE && first + 8 <= count) {
-        float part[W];
+    for (uint64_t first = ((uint64_t)blockIdx.x * kBlock + threadIdx.x) * 8u; first < count; first += stride) {
+        if (WIDE && first + 8 <= count) {
+            float v[8], part[W];
 #pragma unroll
-        for (int k = 0; k < 8 / W; ++k) {
-            load_vector<D, W>(x, first + k * W, part);
+            for (int k = 0; k < 8 / W; ++k) {
+                load_vector<D, W>(x, first + k * W, part);
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[k * W + j] = part[j];
+                for (int j = 0; j < W; ++j) v[k * W + j] = part[j];
+            }
+            dropout_apply<8>(d, seed, first, v);
+#pragma unroll
+            for (int k = 0; k < 8 / W; ++k) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) part[j] = v[k * W + j];
+                store_vector<D, W>(y, first + k * W, part);
+            }
+        } else {
+            const uint32_t kept = dropout_kept<8>(d, seed, first);
+            const uint32_t n = (uint32_t)min((unsigned long long)(count - first), 8ull);
+            for (uint32_t j = 0; j < n; ++j) {
+                float one[1];
+                load_vector<D, 1>(x, first + j, one);
+                one[0] = (kept >> j) & 1u ? rounded_product(one[0], d.scale) : 0.0f;
+                store_vector<D, 1>(y, first + j, one);
+            }
         }
-        dropout_apply<8>(d, seed, first, v);
-#pragma unroll
-        for (int k = 0; k < 8 / W; ++k) {
-#pragma unroll
-            for (int j = 0; j < W; ++j) part[j] = v[k * W + j];
-            store_vector<D, W>(y, first + k * W, part);
-        }
-        return;
-    }
-    const uint32_t kept = dropout_kept<8>(d, seed, first);
-    const uint32_t n = (uint32_t)min((unsigned long long)(count - first), 8ull);
-    for (uint32_t j = 0; j < n; ++j) {
-        float one[1];
-        load_vector<D, 1>(x, first + j, one);
-        one[0] = (kept >> j) & 1u ? rounded_product(one[0], d.scale) : 0.0f;
-        store_vector<D, 1>(y, first + j, one);
     }
 }
 
 template <int D>
 int launch(const void* x, void* y, uint64_t count, const Dropout& d, hipStream_t stream) {
-    const uint32_t blocks = (uint32_t)((count + 8 * kBlock - 1) / (8 * kBlock));
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>((count + 8 * kBlock - 1) / (8 * kBlock), kMostBlocks);
     if (((uintptr_t)x | (uintptr_t)y) % 16 == 0) {
         INPC_LAUNCH("dropout", (k_dropout<D, true>), dim3(blocks), dim3(kBlock), stream, x, y, count, d);
     } else {

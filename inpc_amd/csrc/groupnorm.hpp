@@ -318,8 +318,8 @@ struct Differences {
     // with n values: their sum, and the sum of their squared deviations from `mean`
     __device__ __forceinline__ float sum(int q, float n) const { return fmaf(n, pivot[q], s1[q]); }
     __device__ __forceinline__ float deviations(int q, float n, float share, float mean) const {   // share: 1 / n, or 0
-        const float own = s1[q] * share, d = pivot[q] + own - mean;
-        return fmaf(n * d, d, fmaxf(fmaf(-s1[q], own, s2[q]), 0.0f));
+        const float own = s1[q] * share, d = pivot[q] + own - mean, rest = fmaf(-s1[q], own, s2[q]);
+        return fmaf(n * d, d, rest < 0.0f ? 0.0f : rest);   // a NaN stays one
     }
 };
 
@@ -573,7 +573,7 @@ __device__ __forceinline__ float2 fold_moments(const float2* mine, const Shape& 
     const float share = n > 0.0f ? s1 / n : 0.0f;
     const float mean = lanes_sum(fmaf(n, pivot, s1), lanes) / count, d = pivot + share - mean;
     const float squares = lanes_sum(fmaf(n * d, d, fmaf(-s1, share, s2)), lanes);
-    return make_float2(mean, 1.0f / sqrtf(fmaxf(squares, 0.0f) / count + s.eps));
+    return make_float2(mean, 1.0f / sqrtf((squares < 0.0f ? 0.0f : squares) / count + s.eps));
 }
 
 // ... and the means A and B of the gradient pass
@@ -853,9 +853,9 @@ inline int check_config(const inpc_group_norm_config* cfg, const char* what) {
     // a thread's offset in a block's rows is counted in 32 bits
     if (cfg->input_pixel_stride >= (1u << 19) || cfg->grad_pixel_stride >= (1u << 19))
         return fail(INPC_E_UNSUPPORTED, "%s: pixel strides are below 2^19 elements", what);
-    // blocks are counted in 31 bits
-    if ((uint64_t)cfg->n_images * cfg->groups > 0x7FFFFFFFu || (uint64_t)cfg->n_images + kApplyBlocks > 0x7FFFFFFFu)
-        return fail(INPC_E_UNSUPPORTED, "%s: too many images", what);
+    // a launch has fewer than 2^32 threads: at most a block per (image, group), or for large groups per (image, tile)
+    if ((uint64_t)cfg->n_images * cfg->groups > 0xFFFFFFFFu / kThreads)
+        return fail(INPC_E_UNSUPPORTED, "%s: too many images: at most %u groups in all", what, 0xFFFFFFFFu / kThreads);
     if (!(cfg->eps >= 0.0f)) return fail(INPC_E_INVALID_ARGUMENT, "%s: eps must not be negative", what);
     if (!valid_probability(cfg->dropout_p)) return fail(INPC_E_INVALID_ARGUMENT, "%s: the dropout probability is outside [0, 1]", what);
     return INPC_OK;

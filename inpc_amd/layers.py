@@ -75,6 +75,16 @@ def _dropout_call(x: torch.Tensor, p: float, seed: int, seed_tensor: torch.Tenso
     return out
 
 
+def _dropout_backward(ctx: Any, grad: torch.Tensor):
+    if ctx.random[2] is not None:
+        ctx.saved_tensors   # refuses a seed tensor that has changed
+    return _dropout_call(grad.contiguous(memory_format=ctx.order), *ctx.random), None, None
+
+
+# Under create_graph the result must refuse to be differentiated again; otherwise that wrapper's few microseconds are saved.
+_dropout_backward_once = once_differentiable(_dropout_backward)
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, order: torch.memory_format, random: tuple) -> torch.Tensor:
@@ -84,10 +94,8 @@ class _Dropout(torch.autograd.Function):
         return _dropout_call(x, *random)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):
-        ctx.saved_tensors
-        return _dropout_call(grad.contiguous(memory_format=ctx.order), *ctx.random), None, None
+        return (_dropout_backward_once if torch.is_grad_enabled() else _dropout_backward)(ctx, grad)
 
 
 def dropout(input: torch.Tensor, p: float, seed: int | torch.Tensor | None, offset: int = 0, training: bool = True) -> torch.Tensor:
@@ -173,6 +181,34 @@ def _group_norm_call(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.T
     return y, x, moments, cfg
 
 
+def _require_parameter(t: torch.Tensor, name: str, channels: int, input: torch.Tensor) -> torch.Tensor:
+    if t.dim() != 1 or t.shape[0] != channels:
+        raise ValueError(f"expected {name} of shape ({channels},), got {tuple(t.shape)}")
+    if t.dtype != torch.float32 and t.dtype != input.dtype:
+        raise RuntimeError("weight and bias have one scalar type, Float or that of the input")
+    if t.device != input.device:
+        raise RuntimeError("expected all tensors on the same device")
+    return t.contiguous()
+
+
+def _group_norm_backward(ctx: Any, grad: torch.Tensor):
+    x, weight, bias, moments, _ = ctx.saved_tensors
+    cfg = _lib.GroupNormConfig.from_buffer_copy(ctx.cfg)   # two backward passes of one forward pass may run at once
+    grad, cfg.grad_image_stride, cfg.grad_pixel_stride = _channels_last(grad)
+    need_x, need_weight, need_bias, _ = ctx.needs_input_grad
+    new = torch.empty_like if x.numel() else torch.zeros_like
+    dx = _dense(x) if need_x else None
+    dweight = new(weight) if need_weight else None
+    dbias = new(bias) if need_bias else None
+    workspace, size = _workspace(cfg, 1, x.device)
+    _run("inpc_group_norm_backward", x, C.byref(cfg), grad.data_ptr(), x.data_ptr(), _address(weight), _address(bias),
+         moments.data_ptr(), _address(dx), _address(dweight), _address(dbias), _address(workspace), size)
+    return dx, dweight, dbias, None
+
+
+_group_norm_backward_once = once_differentiable(_group_norm_backward)
+
+
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, options: tuple) -> torch.Tensor:
@@ -181,20 +217,8 @@ class _GroupNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):
-        x, weight, bias, moments, _ = ctx.saved_tensors
-        cfg = _lib.GroupNormConfig.from_buffer_copy(ctx.cfg)   # two backward passes of one forward pass may run at once
-        grad, cfg.grad_image_stride, cfg.grad_pixel_stride = _channels_last(grad)
-        need_x, need_weight, need_bias, _ = ctx.needs_input_grad
-        new = torch.empty_like if x.numel() else torch.zeros_like
-        dx = _dense(x) if need_x else None
-        dweight = new(weight) if need_weight else None
-        dbias = new(bias) if need_bias else None
-        workspace, size = _workspace(cfg, 1, x.device)
-        _run("inpc_group_norm_backward", x, C.byref(cfg), grad.data_ptr(), x.data_ptr(), _address(weight), _address(bias),
-             moments.data_ptr(), _address(dx), _address(dweight), _address(dbias), _address(workspace), size)
-        return dx, dweight, dbias, None
+        return (_group_norm_backward_once if torch.is_grad_enabled() else _group_norm_backward)(ctx, grad)
 
 
 def group_norm(input: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -222,18 +246,14 @@ def group_norm(input: torch.Tensor, num_groups: int, weight: torch.Tensor | None
         raise ValueError(f"unknown activation {activation!r}; choose from {', '.join(_ACTIVATIONS)}")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if t.shape != (channels,):
-            raise ValueError(f"expected {name} of shape ({channels},), got {tuple(t.shape)}")
-        if t.dtype not in (torch.float32, input.dtype) or (weight is not None and bias is not None and weight.dtype != bias.dtype):
+    if weight is not None:
+        weight = _require_parameter(weight, "weight", channels, input)
+    if bias is not None:
+        bias = _require_parameter(bias, "bias", channels, input)
+        if weight is not None and weight.dtype != bias.dtype:
             raise RuntimeError("weight and bias have one scalar type, Float or that of the input")
-        if t.device != input.device:
-            raise RuntimeError("expected all tensors on the same device")
     p = _require_probability(dropout_p, "dropout_p") if training else 0.0
     seed, seed_tensor, offset = _require_seed(seed, offset, input.device) if p > 0.0 else (0, None, 0)
-    weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
     options = num_groups, float(eps), _ACTIVATIONS[activation], p, seed, seed_tensor, offset
     if torch.is_grad_enabled() and (input.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):

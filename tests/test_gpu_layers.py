@@ -317,11 +317,12 @@ def test_group_norm_gradient_against_differences(gpu):
             assert (difference - (got[name].cpu().double() * direction.double()).sum()).abs() <= 1.01 * tolerance + 1e-4, (act, name)
 
 
-def test_group_norm_keeps_what_is_not_finite_inside_its_group(gpu):
-    x, weight, bias, dy = make_case(2, 8, 6, 5, "fp32", 31)
+@pytest.mark.parametrize("size", [(6, 5), (90, 101)], ids=["single", "split"])
+def test_group_norm_keeps_what_is_not_finite_inside_its_group(gpu, size):
+    x, weight, bias, dy = make_case(2, 8, *size, "fp32", 31)
     bad = x.clone()
     bad[0, 1, 2, 3] = float("nan")     # group 0 of image 0
-    bad[1, 6, 0, 0] = float("inf")     # group 3 of image 1
+    bad[1, 6, -1, -1] = float("inf")   # group 3 of image 1
     want = group_norm(to_device(x), 4, to_device(weight), to_device(bias)).cpu()
     got = group_norm(to_device(bad), 4, to_device(weight), to_device(bias)).cpu()
     hit = torch.zeros(2, 8, 1, 1, dtype=torch.bool)

@@ -61,7 +61,10 @@ def config(**changes):
     (dict(dropout_p=float("nan")), -1, b"probability"),
     (dict(channels=131072, groups=1), -3, b"65536"),
     (dict(n_pixels=1 << 30), -3, b"2^30"),
+    (dict(n_images=1 << 23), -3, b"images"),
     (dict(n_images=0xFFFFFFFF, channels=8, groups=8), -3, b"images"),
+    (dict(input_pixel_stride=1 << 19), -3, b"strides"),
+    (dict(grad_pixel_stride=1 << 19), -3, b"strides"),
 ])
 def test_refused_configurations(changes, code, word):
     lib = _lib.lib()

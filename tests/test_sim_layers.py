@@ -1,0 +1,61 @@
+"""group_norm and dropout on the CPU: tests of tests/test_gpu_layers.py called with the simulator's build of the kernels in the HIP
+library's place (tests/cpu_sim; test_sim_kernels.py says what that shows and what not). Both forms of the norm, all types and
+vector widths, the second draw of the generator, refusals; about a minute together. `pytest tests/test_gpu_layers.py -m gpu --sim`
+runs all of them."""
+import importlib
+import inspect
+import os
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+CASES = [
+    ("test_dropout_is_its_definition_bit_for_bit", dict(count=10007, dtype="bf16")),
+    ("test_dropout_is_its_definition_bit_for_bit", dict(count=9, dtype="fp32")),
+    ("test_dropout_second_draw_decides_ties", {}),
+    ("test_dropout_extremes", dict(dtype="fp32")),
+    ("test_dropout_layouts", dict(dtype="fp16")),
+    ("test_dropout_seed_on_the_device", {}),
+    ("test_group_norm", dict(shape=(3, 30, 11, 7, 5), dtype="fp16")),
+    ("test_group_norm", dict(shape=(1, 2064, 3, 2, 1), dtype="fp32")),
+    ("test_group_norm", dict(shape=(5, 4, 1, 1, 2), dtype="bf16")),
+    ("test_group_norm_of_large_groups", dict(shape=(2, 24, 120, 95, 3, "fp16", "gelu", 0.25))),
+    ("test_group_norm_of_large_groups", dict(shape=(1, 33, 200, 200, 33, "fp32", "silu", 0.1))),
+    ("test_group_norm_of_large_groups", dict(shape=(1, 40, 120, 75, 5, "fp32", "relu", 0.0))),
+    ("test_group_norm_activation_and_dropout", dict(act="silu", p=0.35, dtype="bf16")),
+    ("test_group_norm_layouts", dict(dtype="bf16")),
+    ("test_group_norm_of_values_far_from_zero", {}),
+    ("test_group_norm_gradient_against_differences", {}),
+    ("test_group_norm_keeps_what_is_not_finite_inside_its_group", dict(size=(90, 101))),
+    ("test_group_norm_of_nothing", {}),
+    ("test_norm_then_dropout_is_the_chain_of_both", {}),
+    ("test_a_training_step_from_points_to_loss", {}),
+    ("test_refusals", {}),
+]
+
+
+def _case_id(case):
+    name, kwargs = case
+    return name[5:] + "".join(f"-{v}".replace(" ", "") for v in kwargs.values())
+
+
+@pytest.mark.parametrize("case", CASES, ids=_case_id)
+def test_on_the_simulator(sim, case):
+    name, kwargs = case
+    function = getattr(importlib.import_module("tests.test_gpu_layers"), name)
+    assert set(inspect.signature(function).parameters) == {"gpu", *kwargs}
+    assert "real_gpu" not in [m.name for m in getattr(function, "pytestmark", [])]
+    function(gpu=sim, **kwargs)
+
+
+@pytest.mark.parametrize("order", ["reverse", "shuffle"])
+def test_results_do_not_depend_on_the_order_of_threads_and_blocks(order):
+    chosen = [_case_id(c) for c in CASES if "large_groups" in c[0] or c[0] in ("test_group_norm", "test_dropout_layouts")]
+    nodes = [f"{Path(__file__)}::test_on_the_simulator[{case}]" for case in chosen]
+    done = subprocess.run([sys.executable, "-m", "pytest", *nodes, "-q", "-x", "-p", "no:cacheprovider"],
+                          env=dict(os.environ, INPC_SIM_ORDER=order), capture_output=True, text=True, stdin=subprocess.DEVNULL,
+                          timeout=900, cwd=Path(__file__).resolve().parent.parent)
+    assert done.returncode == 0, done.stdout[-3000:] + done.stderr[-2000:]
+    assert f"{len(chosen)} passed" in done.stdout, done.stdout[-2000:]
