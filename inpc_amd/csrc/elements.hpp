@@ -64,6 +64,18 @@ __device__ __forceinline__ void from_words(const uint32_t (&w)[4], uint2& p) { p
 __device__ __forceinline__ void from_words(const uint32_t (&w)[4], uint32_t& p) { p = w[0]; }
 __device__ __forceinline__ void from_words(const uint32_t (&w)[4], uint16_t& p) { p = (uint16_t)w[0]; }
 
+// A store that leaves the caches to what is read again.
+__device__ __forceinline__ void store_streamed(uint4* to, const uint4& p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(words{p.x, p.y, p.z, p.w}, (words*)to);
+#else
+    *to = p;
+#endif
+}
+template <typename T>
+__device__ __forceinline__ void store_streamed(T* to, const T& p) { *to = p; }   // narrower ones are not worth it
+
 template <int D, int V>
 __device__ __forceinline__ void unpack(const PackedVector<D, V>& p, float (&v)[V]) {
     uint32_t w[4] = {0, 0, 0, 0};

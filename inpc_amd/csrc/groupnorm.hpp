@@ -5,12 +5,17 @@
 //   backward: dz = dy * activation'(z);  dbias = sum dz, dweight = sum dz * xhat over images and pixels;
 //   dx = (weight * dz - A - xhat * B) / sqrt(var + eps), A and B the group's means of weight * dz and weight * dz * xhat
 //
-// Two forms. "single": a block per (image, group) does everything in one launch, from registers where the group fits them;
-// for maps whose launches cost more than their bytes. "split": a block per run of pixels (a slab) of an image, all channels
-// of it wide, so that it reads whole runs of memory; one launch writes each slab's sums, the next adds them up at the
-// start of every block and applies. In both a thread keeps one vector of channels (16 bytes where channel counts, strides
+// Two forms. "single": a block per (image, group) does everything in one launch, for small maps, whose launches and latencies
+// cost more than their bytes. "split": a block per run of pixels (a slab) of an image, all channels wide, so that it reads
+// whole runs of memory; one launch writes each slab's sums, the next adds them up at the start of every block (or a
+// launch in between does) and applies. In both a thread keeps one vector of channels (16 bytes where channel counts, strides
 // and pointers allow). Sums are fp32 in an order that depends on sizes and alignments alone (no atomics); deviations are
 // taken from a value of the data, so that nothing cancels however far the values are from 0.
+//
+// What bounds it: memory. Forward reads x twice and writes y, backward reads x and dy twice and writes dx; up to some 200 MB
+// the second read comes from the 256 MB memory-side cache. 1240x824x32 fp16 (65 MB), SiLU: moments 15 us (4.4 TB/s), apply
+// 26 us (5.0 TB/s read and written), gradient sums 28 us (4.7 TB/s), input gradient 36 us (5.5 TB/s); without the activation the
+// gradient sums take 26 us. A plain copy of that size reaches 5.9 TB/s from the cache and 4.9 TB/s from memory.
 #pragma once
 
 #include <algorithm>
@@ -23,12 +28,20 @@ namespace norm {
 
 constexpr int kMaxThreads = 512;         // of the single form
 constexpr int kThreads = 512;            // of the split form
-constexpr int kUnroll = 4;               // vectors a thread has in flight
-constexpr int kUnrollBackward = 2;       // ... of x and of dy each
-constexpr uint32_t kSumBlocks = 512;     // of the split form: two on each compute unit
-constexpr uint32_t kApplyBlocks = 1024;  // ... where sums need not be added up by every block
-constexpr uint32_t kFoldedSums = 4096;   // slab sums of a tile of an image up to which they are
-constexpr uint32_t kTileGroups = 32;     // groups of a tile at most
+// Vectors a thread has in flight, forward, and of x and of dy each, backward. Twice as many in the backward pass cost a wave of
+// occupancy: gradient sums of 65 MB of fp16 31 -> 40 us; half as many change nothing.
+constexpr int kUnroll = 4;
+constexpr int kUnrollBackward = 2;
+// Blocks of a launch that sums: two on each compute unit. With 1024 the blocks' own reductions weigh more (gradient sums of
+// 65 MB 31 -> 37 us); with 256 nothing is gained there (31 us) and an input gradient of as many blocks takes 35 us instead of 32.
+constexpr uint32_t kSumBlocks = 512;
+// Where the sums of a tile of an image are at most this many, every applying block adds them up itself; beyond a launch in
+// between does. 65 MB, 8 groups (4000 sums): apply 27 us against 23 us + 4.4 us and the launch; 33 MB, 32 groups (16000 sums):
+// 26 us against 16 us + 4.5 us.
+constexpr uint32_t kFoldedSums = 4096;
+// Blocks of a launch that applies and does not add up. 65 MB: 22.7 us with 1024, 23.4 with 2048, 27.9 with 4096.
+constexpr uint32_t kApplyBlocks = 1024;
+constexpr uint32_t kTileGroups = 32;     // groups of a tile of channels at most: a block's threads share them out at once
 constexpr uint32_t kParameterColumns = 32;
 
 struct Shape {
@@ -40,6 +53,7 @@ struct Shape {
     uint32_t slabs, slab_pixels; // ... and runs of pixels of each tile of an image
     int32_t activation, param_dtype;
     float eps;
+    bool streamed;               // split form: the result is stored past the caches
 };
 
 // f(0), ..., f(N - 1) written out with constant arguments: an array indexed by them stays in registers, which a loop that the
@@ -175,12 +189,13 @@ struct Rows {
     char* base;
     uint64_t step;   // bytes
     uint32_t lane;   // bytes
+    bool streamed;   // stores go past the caches
 };
 // `first`: the element that the run's first pixel and the block's first channel make
 template <int D, int V>
 __device__ __forceinline__ Rows rows_of(const void* map, uint64_t first, uint64_t pixel_stride, const Shape& s) {
     return Rows{(char*)map + first * kElementBytes<D>, s.rows * pixel_stride * kElementBytes<D>,
-                (uint32_t)((threadIdx.x / s.columns * (uint32_t)pixel_stride + threadIdx.x % s.columns * V) * kElementBytes<D>)};
+                (uint32_t)((threadIdx.x / s.columns * (uint32_t)pixel_stride + threadIdx.x % s.columns * V) * kElementBytes<D>), false};
 }
 template <int D, int V>
 __device__ __forceinline__ PackedVector<D, V> load_row(const Rows& m, uint32_t k, uint32_t skip = 0) {
@@ -189,7 +204,9 @@ __device__ __forceinline__ PackedVector<D, V> load_row(const Rows& m, uint32_t k
 
 template <int D, int V>
 __device__ __forceinline__ void store_row(const Rows& m, uint32_t k, uint32_t skip, const float (&v)[V]) {
-    *(PackedVector<D, V>*)(m.base + k * m.step + (m.lane + skip * kElementBytes<D>)) = pack<D, V>(v);
+    auto* to = (PackedVector<D, V>*)(m.base + k * m.step + (m.lane + skip * kElementBytes<D>));
+    if (m.streamed) store_streamed(to, pack<D, V>(v));
+    else *to = pack<D, V>(v);
 }
 
 // The same for element numbers: of the result, which is dense
@@ -255,8 +272,8 @@ __device__ __forceinline__ Rows shifted(Rows m, uint32_t skip) {
     return m;
 }
 
-// f(k, vector k of the map, or of both) for all vectors that a thread has in a run of `size` pixels: N at a time, loaded before the first is used. `k` is
-// the same for the whole block.
+// f(k, vector k of the map, or of both) for all vectors that a thread has in a run of `size` pixels: N at a time, loaded before
+// the first is used. `k` is the same for the whole block.
 template <int D, int V, int N, typename F>
 __device__ __forceinline__ void stream(const Rows& x, uint32_t rows, uint32_t size, uint32_t row, F f) {
     if (row >= size) return;
@@ -289,7 +306,7 @@ __device__ __forceinline__ void stream(const Rows& x, const Rows& g, uint32_t ro
 
 // A thread's sums of differences from its first value, for each slot of its vectors. N values with a common pivot that is one of
 // them: the pivot's squared distance from the group's mean is at most the group's sum of squared deviations, so that what cancels
-// in s2 - s1^2 / N costs at most a factor of N (some hundred) in the last place.
+// in s2 - s1^2 / N costs at most a factor of N in the last place (hundreds, where that one value makes up the whole variance).
 template <int V, int Q>
 struct Differences {
     float pivot[Q], s1[Q], s2[Q];
@@ -645,7 +662,8 @@ __global__ void __launch_bounds__(kThreads) k_apply(const void* __restrict__ x, 
     if (row >= p.size) return;
     const Affine<V, Q> a = load_affine<V, Q>(s, m, p.channel, p.channel + threadIdx.x % s.columns * V, weight, bias);
     const uint64_t seed = dropout_seed(d);
-    const Rows ry = rows_at<D, V>(y, p, (uint64_t)s.pixels * s.channels, s.channels, s);
+    Rows ry = rows_at<D, V>(y, p, (uint64_t)s.pixels * s.channels, s.channels, s);
+    ry.streamed = s.streamed;
     const Numbers numbers = numbers_at<V>(p, s);
     stream<D, V, kUnroll>(rows_at<D, V>(x, p, s.x_image, s.x_pixel, s), s.rows, p.size, row, [&](uint32_t k, const PackedVector<D, V>& packed) {
         apply_vector<D, V, Q>(s, d, seed, a, packed, ry, numbers, k);
@@ -669,8 +687,8 @@ __global__ void __launch_bounds__(kThreads) k_gradient_sums(const void* __restri
         const Affine<V, Q> a = load_affine<V, Q>(s, moments, 0, p.channel + threadIdx.x % s.columns * V, weight, bias);
         const uint64_t seed = dropout_seed(d);
         const Numbers numbers = numbers_at<V>(p, s);
-        stream<D, V, kUnrollBackward>(rows_at<D, V>(x, p, s.x_image, s.x_pixel, s), rows_at<D, V>(dy, p, s.g_image, s.g_pixel, s), s.rows, p.size, row,
-                                      [&](uint32_t k, const PackedVector<D, V>& px, const PackedVector<D, V>& pg) {
+        stream<D, V, kUnrollBackward>(rows_at<D, V>(x, p, s.x_image, s.x_pixel, s), rows_at<D, V>(dy, p, s.g_image, s.g_pixel, s),
+                                      s.rows, p.size, row, [&](uint32_t k, const PackedVector<D, V>& px, const PackedVector<D, V>& pg) {
                                           float v[V], g[V];
                                           gradient_vector<D, V, Q>(s, d, seed, a, px, pg, number_of(numbers, k), v, g);
 #pragma unroll
@@ -737,10 +755,11 @@ __global__ void __launch_bounds__(kThreads) k_input_gradient(const void* __restr
         k2[q] = v.y * a.rstd[q] * a.rstd[q];
     }
     const uint64_t seed = dropout_seed(d);
-    const Rows rdx = rows_at<D, V>(dx, p, (uint64_t)s.pixels * s.channels, s.channels, s);
+    Rows rdx = rows_at<D, V>(dx, p, (uint64_t)s.pixels * s.channels, s.channels, s);
+    rdx.streamed = s.streamed;
     const Numbers numbers = numbers_at<V>(p, s);
-    stream<D, V, kUnrollBackward>(rows_at<D, V>(x, p, s.x_image, s.x_pixel, s), rows_at<D, V>(dy, p, s.g_image, s.g_pixel, s), s.rows, p.size, row,
-                                  [&](uint32_t k, const PackedVector<D, V>& px, const PackedVector<D, V>& pg) {
+    stream<D, V, kUnrollBackward>(rows_at<D, V>(x, p, s.x_image, s.x_pixel, s), rows_at<D, V>(dy, p, s.g_image, s.g_pixel, s),
+                                  s.rows, p.size, row, [&](uint32_t k, const PackedVector<D, V>& px, const PackedVector<D, V>& pg) {
                                       input_gradient_vector<D, V, Q>(s, d, seed, a, k1, k2, px, pg, rdx, numbers, k);
                                   });
 }
@@ -772,7 +791,9 @@ inline Shape base_shape(const inpc_group_norm_config& cfg) {
     return s;
 }
 
-// Bytes of one group of one image up to which the single form runs.
+// Bytes of one group of one image up to which the single form runs. Forward + backward, kernels alone: groups of 16 KB (39x26x256
+// bf16, 8 images) single 9 + 16 us, split 14 + 24 us; of 64 KB (64x64x32 fp32) 12 + 23 against 12 + 17 us; of 93 KB
+// (77x101x30 bf16, 3 images) 19 + 30 against 10 + 12 us.
 constexpr uint64_t kSingleBytes = 32 * 1024;
 
 // Groups of a tile of the split form with vectors of v elements: as many as fit, with boundaries on vectors' boundaries; 0 where
@@ -813,6 +834,16 @@ inline Shape split_shape(const inpc_group_norm_config& cfg, int v, uint32_t bloc
     s.slab_pixels = (uint32_t)((wanted + step - 1) / step * step);
     s.slabs = div_up(s.pixels, s.slab_pixels);
     return s;
+}
+
+// Where a call's maps together (x and y, or x, dy and dx) are larger than this, the result is stored past the caches: what it
+// would push out of the 256 MB memory-side cache is the map that is read for the second time. Maps of 130 MB: forward 87 -> 73 us,
+// backward 149 -> 128 us, also with an operator behind it that reads y (124 -> 121 us); of 65 MB and less nothing is gained, and
+// that next operator finds less of y in the cache (62.4 -> 62.8 us).
+constexpr uint64_t kStreamedBytes = 192ull << 20;
+
+inline bool streams(const inpc_group_norm_config& cfg, int maps) {
+    return (uint64_t)cfg.n_images * cfg.n_pixels * cfg.channels * element_bytes(cfg.dtype) * maps > kStreamedBytes;
 }
 
 inline bool folds(const Shape& s) { return (uint64_t)s.slabs * s.tile_groups <= kFoldedSums; }
@@ -911,7 +942,7 @@ int backward_single(const inpc_group_norm_config& cfg, const void* x, const void
         if ((per_group) % V == 0) {                                                    \
             __VA_ARGS__((k<D, V, 1>))                                                  \
         } else if (V > 2 && (per_group) * 2 == V) {                                    \
-            __VA_ARGS__((k<D, V, V < 4 ? V : 2>))                                      \
+            __VA_ARGS__((k<D, V, (V > 2 ? 2 : V)>))                                      \
         } else {                                                                       \
             __VA_ARGS__((k<D, V, V>))                                                  \
         }                                                                              \
@@ -930,7 +961,8 @@ int forward_split(const inpc_group_norm_config& cfg, const void* x, const void* 
     if (!fold)
         INPC_LAUNCH("group_norm_combine_moments", k_combine_moments, dim3(div_up(s.n * s.groups, kThreads / 64)), dim3(kThreads), stream,
                     partial, moments, s);
-    const Shape a = fold ? s : split_shape(cfg, V, kApplyBlocks);
+    Shape a = fold ? s : split_shape(cfg, V, kApplyBlocks);
+    a.streamed = streams(cfg, 2);
     const float2* to_fold = fold ? partial : nullptr;
 #define INPC_NORM_APPLY(k)                                                                                                              \
     INPC_LAUNCH("group_norm_apply", k, dim3(a.n * a.tiles * a.slabs), dim3(kThreads), stream, x, to_fold, weight, bias, y, moments, a, d);
@@ -959,7 +991,8 @@ int backward_split(const inpc_group_norm_config& cfg, const void* x, const void*
                     dim3(parameter_blocks + (dx ? div_up(s.n * s.groups, kThreads / 64) : 0)), dim3(kThreads), stream, of_groups,
                     of_channels, means, dweight, dbias, parameter_blocks, s);
     if (!dx) return INPC_OK;
-    const Shape a = fold ? s : split_shape(cfg, V, kApplyBlocks);
+    Shape a = fold ? s : split_shape(cfg, V, kApplyBlocks);
+    a.streamed = streams(cfg, 3);
     const uint32_t first_blocks = fold ? parameter_blocks : 0;
     const float2* combined = fold ? nullptr : means;
 #define INPC_NORM_GRADIENT(k)                                                                                                       \

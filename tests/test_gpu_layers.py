@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from inpc_amd import dropout, fused_cauchy_loss, group_norm, rasterize_points, synthetic
+from inpc_amd import _lib, dropout, fused_cauchy_loss, group_norm, rasterize_points, synthetic
 from tests import helpers as H
 from tests import layer_reference as R
 
@@ -118,6 +118,15 @@ def test_dropout_seed_on_the_device(gpu):
         held += 1   # the mask of a backward pass could no longer be computed again
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+def test_dropout_in_place_through_the_c_abi(gpu, offset):
+    x = torch.randn(6001, generator=torch.Generator().manual_seed(2)).half()
+    held = to_device(x)[offset:]
+    _lib.check(_lib.lib().inpc_dropout(_lib.ptr(held), _lib.ptr(held), held.numel(), _lib.DTYPE_F16, 0.3, 8, None, 0, H.stream()),
+               "inpc_dropout")
+    assert torch.equal(held.cpu(), R.dropout(x[offset:], 0.3, 8))
 
 
 # ---- group norm ----------------------------------------------------------------------------------------------------
