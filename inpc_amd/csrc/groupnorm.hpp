@@ -35,10 +35,13 @@ constexpr int kUnrollBackward = 2;
 // Blocks of a launch that sums: two on each compute unit. With 1024 the blocks' own reductions weigh more (gradient sums of
 // 65 MB 31 -> 37 us); with 256 nothing is gained there (31 us) and an input gradient of as many blocks takes 35 us instead of 32.
 constexpr uint32_t kSumBlocks = 512;
+// Maps of up to 48 MB take half as many, which leaves fewer sums to add up: moments of 33 MB 13.4 -> 11.2 us, of 16 MB 6.7 -> 6.9.
+constexpr uint32_t kSmallSumBlocks = 256;
+constexpr uint64_t kSmallMap = 48ull << 20;
 // Where the sums of a tile of an image are at most this many, every applying block adds them up itself; beyond a launch in
-// between does. 65 MB, 8 groups (4000 sums): apply 27 us against 23 us + 4.4 us and the launch; 33 MB, 32 groups (16000 sums):
-// 26 us against 16 us + 4.5 us.
-constexpr uint32_t kFoldedSums = 4096;
+// between does. 65 MB, 8 groups (4000 sums): apply 27 us against 23 us + 4.4 us; 33 MB, 32 groups (8000 sums): 20 us against
+// 16 us + 4.5 us, and a launch less for the host; the same with 16000 sums: 26 us against 16 us + 4.5 us.
+constexpr uint32_t kFoldedSums = 8192;
 // Blocks of a launch that applies and does not add up. 65 MB: 22.7 us with 1024, 23.4 with 2048, 27.9 with 4096.
 constexpr uint32_t kApplyBlocks = 1024;
 constexpr uint32_t kTileGroups = 32;     // groups of a tile of channels at most: a block's threads share them out at once
@@ -648,13 +651,13 @@ __global__ void __launch_bounds__(kThreads) k_combine_gradients(const float2* __
 template <int D, int V, int Q>
 __global__ void __launch_bounds__(kThreads) k_apply(const void* __restrict__ x, const float2* __restrict__ partial,
                                                     const void* __restrict__ weight, const void* __restrict__ bias,
-                                                    void* __restrict__ y, float2* __restrict__ moments, Shape s, Dropout d) {
+                                                    void* __restrict__ y, float2* __restrict__ moments, Shape s, Shape of_sums, Dropout d) {
     __shared__ float2 folded[kTileGroups];
     const Place p = place_of(s, blockIdx.x);
     float2* of_tile = moments + (size_t)p.image * s.groups + p.tile * s.tile_groups;
     const float2* m = of_tile;
     if (partial) {
-        fold_tile(partial, s, p, folded, fold_moments);
+        fold_tile(partial, of_sums, p, folded, fold_moments);
         if (p.slab == 0 && threadIdx.x < groups_of_tile(s, p.tile)) of_tile[threadIdx.x] = folded[threadIdx.x];
         m = folded;
     }
@@ -731,17 +734,17 @@ __global__ void __launch_bounds__(kThreads) k_input_gradient(const void* __restr
                                                              const float2* __restrict__ of_groups, const float2* __restrict__ means,
                                                              const void* __restrict__ weight, const void* __restrict__ bias,
                                                              void* __restrict__ dx, void* __restrict__ dweight,
-                                                             void* __restrict__ dbias, uint32_t parameter_blocks, Shape s, Dropout d) {
+                                                             void* __restrict__ dbias, uint32_t parameter_blocks, Shape s, Shape of_sums, Dropout d) {
     __shared__ float lds[column_floats<2>(kThreads)];
     __shared__ float2 folded[kTileGroups];
     if (blockIdx.x < parameter_blocks) {
-        add_parameter_gradients(of_channels, s.n * s.slabs, dweight, dbias, s, blockIdx.x, lds);
+        add_parameter_gradients(of_channels, s.n * of_sums.slabs, dweight, dbias, s, blockIdx.x, lds);
         return;
     }
     const Place p = place_of(s, blockIdx.x - parameter_blocks);
     const float2* ab = means + (size_t)p.image * s.groups + p.tile * s.tile_groups;
     if (!means) {
-        fold_tile(of_groups, s, p, folded, fold_gradients);
+        fold_tile(of_groups, of_sums, p, folded, fold_gradients);
         ab = folded;
     }
     const uint32_t row = thread_row(s, p, V), channel = p.channel + threadIdx.x % s.columns * V;
@@ -792,9 +795,9 @@ inline Shape base_shape(const inpc_group_norm_config& cfg) {
 }
 
 // Bytes of one group of one image up to which the single form runs. Forward + backward, kernels alone: groups of 16 KB (39x26x256
-// bf16, 8 images) single 9 + 16 us, split 14 + 24 us; of 64 KB (64x64x32 fp32) 12 + 23 against 12 + 17 us; of 93 KB
-// (77x101x30 bf16, 3 images) 19 + 30 against 10 + 12 us.
-constexpr uint64_t kSingleBytes = 32 * 1024;
+// bf16, 8 images) single 9 + 16 us, split 14 + 24 us; of 64 KB (64x64x32 fp32) 12 + 23 against 12 + 17 us, with two launches less,
+// so that a step as a whole takes 107 against 120 us; of 93 KB (77x101x30 bf16, 3 images) 19 + 30 against 10 + 12 us.
+constexpr uint64_t kSingleBytes = 64 * 1024;
 
 // Groups of a tile of the split form with vectors of v elements: as many as fit, with boundaries on vectors' boundaries; 0 where
 // not even the fewest do.
@@ -822,7 +825,11 @@ inline Shape single_shape(const inpc_group_norm_config& cfg, int v, uint32_t& th
     return s;
 }
 
-inline Shape split_shape(const inpc_group_norm_config& cfg, int v, uint32_t blocks = kSumBlocks) {
+inline uint64_t map_bytes(const inpc_group_norm_config& cfg) {
+    return (uint64_t)cfg.n_images * cfg.n_pixels * cfg.channels * element_bytes(cfg.dtype);
+}
+
+inline Shape split_shape(const inpc_group_norm_config& cfg, int v, uint32_t blocks) {
     Shape s = base_shape(cfg);
     s.tile_groups = tile_groups_of(cfg, v);
     s.tiles = div_up(s.groups, s.tile_groups);
@@ -836,6 +843,10 @@ inline Shape split_shape(const inpc_group_norm_config& cfg, int v, uint32_t bloc
     return s;
 }
 
+inline Shape sums_shape(const inpc_group_norm_config& cfg, int v) {
+    return split_shape(cfg, v, map_bytes(cfg) <= kSmallMap ? kSmallSumBlocks : kSumBlocks);
+}
+
 // Where a call's maps together (x and y, or x, dy and dx) are larger than this, the result is stored past the caches: what it
 // would push out of the 256 MB memory-side cache is the map that is read for the second time. Maps of 130 MB: forward 87 -> 73 us,
 // backward 149 -> 128 us, also with an operator behind it that reads y (124 -> 121 us); of 65 MB and less nothing is gained, and
@@ -843,7 +854,7 @@ inline Shape split_shape(const inpc_group_norm_config& cfg, int v, uint32_t bloc
 constexpr uint64_t kStreamedBytes = 192ull << 20;
 
 inline bool streams(const inpc_group_norm_config& cfg, int maps) {
-    return (uint64_t)cfg.n_images * cfg.n_pixels * cfg.channels * element_bytes(cfg.dtype) * maps > kStreamedBytes;
+    return map_bytes(cfg) * maps > kStreamedBytes;
 }
 
 inline bool folds(const Shape& s) { return (uint64_t)s.slabs * s.tile_groups <= kFoldedSums; }
@@ -866,7 +877,7 @@ inline size_t workspace_bytes(const inpc_group_norm_config& cfg, bool backward) 
     size_t most = backward && cfg.n_images > 1 ? (size_t)cfg.n_images * cfg.channels * sizeof(float2) : 0;
     for (int v = (int)(16 / element_bytes(cfg.dtype)); v >= 1; v /= 2)
         if (cfg.channels % (uint32_t)v == 0 && !runs_single(cfg, v))
-            most = std::max(most, split_workspace(split_shape(cfg, v), backward).bytes);
+            most = std::max(most, split_workspace(sums_shape(cfg, v), backward).bytes);
     return most;
 }
 
@@ -951,7 +962,7 @@ int backward_single(const inpc_group_norm_config& cfg, const void* x, const void
 template <int D, int V>
 int forward_split(const inpc_group_norm_config& cfg, const void* x, const void* weight, const void* bias, void* y, float2* moments,
                   char* ws, hipStream_t stream) {
-    const Shape s = split_shape(cfg, V);
+    const Shape s = sums_shape(cfg, V);
     const Dropout d = make_dropout(cfg.dropout_p, cfg.seed, cfg.seed_dev, cfg.offset);
     float2* partial = (float2*)(ws + split_workspace(s, false).of_groups);
 #define INPC_NORM_MOMENTS(k) INPC_LAUNCH("group_norm_moments", k, dim3(s.n * s.tiles * s.slabs), dim3(kThreads), stream, x, partial, s);
@@ -961,11 +972,11 @@ int forward_split(const inpc_group_norm_config& cfg, const void* x, const void* 
     if (!fold)
         INPC_LAUNCH("group_norm_combine_moments", k_combine_moments, dim3(div_up(s.n * s.groups, kThreads / 64)), dim3(kThreads), stream,
                     partial, moments, s);
-    Shape a = fold ? s : split_shape(cfg, V, kApplyBlocks);
+    Shape a = split_shape(cfg, V, fold ? kSumBlocks : kApplyBlocks);
     a.streamed = streams(cfg, 2);
     const float2* to_fold = fold ? partial : nullptr;
 #define INPC_NORM_APPLY(k)                                                                                                              \
-    INPC_LAUNCH("group_norm_apply", k, dim3(a.n * a.tiles * a.slabs), dim3(kThreads), stream, x, to_fold, weight, bias, y, moments, a, d);
+    INPC_LAUNCH("group_norm_apply", k, dim3(a.n * a.tiles * a.slabs), dim3(kThreads), stream, x, to_fold, weight, bias, y, moments, a, s, d);
     INPC_NORM_SLOTS(k_apply, s.per_group, INPC_NORM_APPLY);
 #undef INPC_NORM_APPLY
     return INPC_OK;
@@ -974,7 +985,7 @@ int forward_split(const inpc_group_norm_config& cfg, const void* x, const void* 
 template <int D, int V>
 int backward_split(const inpc_group_norm_config& cfg, const void* x, const void* dy, const float2* moments, const void* weight,
                    const void* bias, void* dx, void* dweight, void* dbias, char* ws, hipStream_t stream) {
-    const Shape s = split_shape(cfg, V);
+    const Shape s = sums_shape(cfg, V);
     const Dropout d = make_dropout(cfg.dropout_p, cfg.seed, cfg.seed_dev, cfg.offset);
     const Workspace w = split_workspace(s, true);
     float2 *of_groups = (float2*)(ws + w.of_groups), *of_channels = (float2*)(ws + w.of_channels), *means = (float2*)(ws + w.means);
@@ -991,13 +1002,13 @@ int backward_split(const inpc_group_norm_config& cfg, const void* x, const void*
                     dim3(parameter_blocks + (dx ? div_up(s.n * s.groups, kThreads / 64) : 0)), dim3(kThreads), stream, of_groups,
                     of_channels, means, dweight, dbias, parameter_blocks, s);
     if (!dx) return INPC_OK;
-    Shape a = fold ? s : split_shape(cfg, V, kApplyBlocks);
+    Shape a = split_shape(cfg, V, fold ? kSumBlocks : kApplyBlocks);
     a.streamed = streams(cfg, 3);
     const uint32_t first_blocks = fold ? parameter_blocks : 0;
     const float2* combined = fold ? nullptr : means;
 #define INPC_NORM_GRADIENT(k)                                                                                                       \
     INPC_LAUNCH("group_norm_input_gradient", k, dim3(first_blocks + a.n * a.tiles * a.slabs), dim3(kThreads), stream, x, dy, moments, \
-                of_channels, of_groups, combined, weight, bias, dx, dweight, dbias, first_blocks, a, d);
+                of_channels, of_groups, combined, weight, bias, dx, dweight, dbias, first_blocks, a, s, d);
     INPC_NORM_SLOTS(k_input_gradient, s.per_group, INPC_NORM_GRADIENT);
 #undef INPC_NORM_GRADIENT
     return INPC_OK;

@@ -92,8 +92,8 @@ class GroupNorm:
         D = 32 + 8 * per_group + 256 / per_group
         split = lambda t: t.double().permute(0, 2, 3, 1).reshape(n, h * w, groups, per_group)  # noqa: E731
         whole = lambda t: t.reshape(n, h, w, c).permute(0, 3, 1, 2)  # noqa: E731
-        wt = (torch.ones(c) if weight is None else weight).double().view(groups, per_group)
-        bs = (torch.zeros(c) if bias is None else bias).double().view(groups, per_group)
+        wt = (x.new_ones(c) if weight is None else weight).double().view(groups, per_group)
+        bs = (x.new_zeros(c) if bias is None else bias).double().view(groups, per_group)
         param = next((t.dtype for t in (weight, bias) if t is not None), torch.float32)
         v = split(x)
         mean = v.mean(dim=(1, 3), keepdim=True)
@@ -132,7 +132,7 @@ class GroupNorm:
 
 
 def assert_within(got: torch.Tensor, want: torch.Tensor, bound: torch.Tensor, what: str) -> None:
-    off = (got.detach().cpu().double() - want).abs()
+    off = (got.detach().to(want.device).double() - want).abs()
     bad = ~(off <= bound)
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} values outside their bound; worst {float((off / bound).max()):.3g} "
                            f"times it")

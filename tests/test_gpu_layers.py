@@ -207,7 +207,7 @@ SPLIT_SHAPES = [
     (2, 24, 120, 95, 3, "fp32", "silu", 0.25),
     (3, 6, 210, 113, 2, "bf16", "silu", 0.5),       # vectors of two, 170 rows to a block
     (1, 40, 120, 75, 5, "fp32", "relu", 0.0),
-    (1, 33, 200, 200, 33, "fp32", "silu", 0.1),     # single elements, more slab sums than every block adds up itself
+    (1, 33, 200, 200, 33, "fp32", "silu", 0.1),     # single elements, two tiles of channels, the second of one group
     (1, 640, 41, 13, 2, "fp16", "none", 0.0),       # 80 columns, 320 channels to a group
 ]
 
@@ -216,6 +216,20 @@ SPLIT_SHAPES = [
 def test_group_norm_of_large_groups(gpu, shape):
     *size, groups, dtype, act, p = shape
     check(*make_case(*size, dtype, sum(size)), groups, act, p=p, seed=19)
+
+
+def test_group_norm_some_gradients_of_large_groups(gpu):
+    x, weight, bias, dy = make_case(2, 8, 100, 90, "fp32", 77)
+    ref = R.GroupNorm(x, 2, weight, bias, 1e-5, "silu", None, dy)
+    for wanted in ("x", "weight", "bias", "x bias"):
+        leaves = {name: to_device(t).requires_grad_(name in wanted.split())
+                  for name, t in (("x", x), ("weight", weight), ("bias", bias))}
+        group_norm(leaves["x"], 2, leaves["weight"], leaves["bias"], activation="silu").backward(to_device(dy))
+        for name, t in leaves.items():
+            if name in wanted.split():
+                R.assert_within(t.grad, getattr(ref, "d" + name), getattr(ref, f"d{name}_bound"), f"d{name} of {wanted}")
+            else:
+                assert t.grad is None
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
@@ -560,3 +574,19 @@ def test_more_than_two_to_the_32_values(gpu):
         ref = R.activation(z, "silu") * keep.permute(2, 0, 1) * 2.0
         # moments of 16.8 million pixels: a chain of up to 2^12 roundings, and half a step of bf16
         R.assert_within(y[-1, 16 * group:16 * group + 16, -rows:], ref, 4096 * R.U * (z.abs() + 1) + 2.0**-8 * ref.abs(), "y")
+
+
+@pytest.mark.real_gpu
+def test_a_map_beyond_the_caches(gpu):
+    """A map of 102 MB in 20 groups: more slab sums than every block adds up itself, and results that are stored past the caches."""
+    gen = torch.Generator(device=gpu).manual_seed(3)
+    x, dy = (torch.randn(1, 800, 800, 40, generator=gen, device=gpu).permute(0, 3, 1, 2) for _ in range(2))
+    weight, bias = (torch.randn(40, generator=gen, device=gpu) for _ in range(2))
+    leaves = [t.requires_grad_(True) for t in (x, weight, bias)]
+    y = group_norm(x, 20, weight, bias, activation="silu")
+    grads = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        ref = R.GroupNorm(x, 20, weight, bias, 1e-5, "silu", None, dy)
+        R.assert_within(y, ref.y, ref.y_bound, "y")
+        for got, name in zip(grads, ("dx", "dweight", "dbias")):
+            R.assert_within(got, getattr(ref, name), getattr(ref, name + "_bound"), name)
