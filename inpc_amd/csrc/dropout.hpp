@@ -14,49 +14,53 @@ namespace inpc {
 namespace dropout {
 
 constexpr int kBlock = 256;
-constexpr uint64_t kMostBlocks = 1u << 20;   // a launch has fewer than 2^32 threads: beyond 2^31 values a thread takes several vectors
+constexpr uint64_t kLaunch = 1ull << 32;   // values of a launch, which has fewer than 2^32 threads
 
-// A thread takes eight consecutive elements, one draw of the generator. WIDE: both pointers are 16-byte aligned.
+// A thread takes eight consecutive elements, one draw of the generator. WIDE: both pointers are 16-byte aligned. No loop over
+// vectors: one costs a tenth (65 MB 20.6 -> 22.7 us).
 template <int D, bool WIDE>
-__global__ void __launch_bounds__(kBlock) k_dropout(const void* x, void* y, uint64_t count, Dropout d) {
-    const uint64_t seed = dropout_seed(d), stride = (uint64_t)gridDim.x * kBlock * 8u;
+__global__ void __launch_bounds__(kBlock) k_dropout(const void* x, void* y, uint64_t begin, uint64_t count, Dropout d) {
+    const uint64_t first = begin + ((uint64_t)blockIdx.x * kBlock + threadIdx.x) * 8u;
+    if (first >= count) return;
+    const uint64_t seed = dropout_seed(d);
     constexpr int W = D == INPC_DTYPE_F32 ? 4 : 8;
-    for (uint64_t first = ((uint64_t)blockIdx.x * kBlock + threadIdx.x) * 8u; first < count; first += stride) {
-        if (WIDE && first + 8 <= count) {
-            float v[8], part[W];
+    if (WIDE && first + 8 <= count) {
+        float v[8], part[W];
 #pragma unroll
-            for (int k = 0; k < 8 / W; ++k) {
-                load_vector<D, W>(x, first + k * W, part);
+        for (int k = 0; k < 8 / W; ++k) {
+            load_vector<D, W>(x, first + k * W, part);
 #pragma unroll
-                for (int j = 0; j < W; ++j) v[k * W + j] = part[j];
-            }
-            dropout_apply<8>(d, seed, first, v);
-#pragma unroll
-            for (int k = 0; k < 8 / W; ++k) {
-#pragma unroll
-                for (int j = 0; j < W; ++j) part[j] = v[k * W + j];
-                store_vector<D, W>(y, first + k * W, part);
-            }
-        } else {
-            const uint32_t kept = dropout_kept<8>(d, seed, first);
-            const uint32_t n = (uint32_t)min((unsigned long long)(count - first), 8ull);
-            for (uint32_t j = 0; j < n; ++j) {
-                float one[1];
-                load_vector<D, 1>(x, first + j, one);
-                one[0] = (kept >> j) & 1u ? rounded_product(one[0], d.scale) : 0.0f;
-                store_vector<D, 1>(y, first + j, one);
-            }
+            for (int j = 0; j < W; ++j) v[k * W + j] = part[j];
         }
+        dropout_apply<8>(d, seed, first, v);
+#pragma unroll
+        for (int k = 0; k < 8 / W; ++k) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) part[j] = v[k * W + j];
+            store_vector<D, W>(y, first + k * W, part);
+        }
+        return;
+    }
+    const uint32_t kept = dropout_kept<8>(d, seed, first);
+    const uint32_t n = (uint32_t)min((unsigned long long)(count - first), 8ull);
+    for (uint32_t j = 0; j < n; ++j) {
+        float one[1];
+        load_vector<D, 1>(x, first + j, one);
+        one[0] = (kept >> j) & 1u ? rounded_product(one[0], d.scale) : 0.0f;
+        store_vector<D, 1>(y, first + j, one);
     }
 }
 
 template <int D>
 int launch(const void* x, void* y, uint64_t count, const Dropout& d, hipStream_t stream) {
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>((count + 8 * kBlock - 1) / (8 * kBlock), kMostBlocks);
-    if (((uintptr_t)x | (uintptr_t)y) % 16 == 0) {
-        INPC_LAUNCH("dropout", (k_dropout<D, true>), dim3(blocks), dim3(kBlock), stream, x, y, count, d);
-    } else {
-        INPC_LAUNCH("dropout", (k_dropout<D, false>), dim3(blocks), dim3(kBlock), stream, x, y, count, d);
+    const bool wide = ((uintptr_t)x | (uintptr_t)y) % 16 == 0;
+    for (uint64_t begin = 0; begin < count; begin += kLaunch) {
+        const dim3 blocks((uint32_t)((std::min(count - begin, kLaunch) + 8 * kBlock - 1) / (8 * kBlock)));
+        if (wide) {
+            INPC_LAUNCH("dropout", (k_dropout<D, true>), blocks, dim3(kBlock), stream, x, y, begin, count, d);
+        } else {
+            INPC_LAUNCH("dropout", (k_dropout<D, false>), blocks, dim3(kBlock), stream, x, y, begin, count, d);
+        }
     }
     return INPC_OK;
 }
