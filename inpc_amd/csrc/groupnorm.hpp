@@ -795,8 +795,8 @@ inline Shape base_shape(const inpc_group_norm_config& cfg) {
 }
 
 // Bytes of one group of one image up to which the single form runs. Forward + backward, kernels alone: groups of 16 KB (39x26x256
-// bf16, 8 images) single 9 + 16 us, split 14 + 24 us; of 64 KB (64x64x32 fp32) 12 + 23 against 12 + 17 us, with two launches less,
-// so that a step as a whole takes 107 against 120 us; of 93 KB (77x101x30 bf16, 3 images) 19 + 30 against 10 + 12 us.
+// bf16, 8 images) single 9 + 16 us, split 14 + 24 us; of 64 KB (64x64x32 fp32) 13 + 21 against 12 + 17 us, with two launches less,
+// so that a step as a whole takes 107 to 113 against 120 us; of 93 KB (77x101x30 bf16, 3 images) 19 + 30 against 10 + 12 us.
 constexpr uint64_t kSingleBytes = 64 * 1024;
 
 // Groups of a tile of the split form with vectors of v elements: as many as fit, with boundaries on vectors' boundaries; 0 where

@@ -228,11 +228,11 @@ def group_norm(input: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     dropout where dropout_p > 0; differentiable in `input`, `weight` and `bias`.
 
     The kernels work on channels-last maps (torch.channels_last, also a slice of the channels of a wider one); other
-    layouts are copied into that first. The result is a dense channels-last tensor of the input's type. `weight`
-    and `bias` are (C,) tensors of one type, fp32 or the input's, so fp32 parameters serve 16-bit maps. Everything is computed in fp32 and rounded
-    once, at the end of the whole chain. `dropout_p`, `seed`, `offset` and `training` are those of `dropout`, which
-    gives the same mask for the same map. For the backward pass only the input and two numbers per image
-    and group are kept.
+    layouts are copied into that first. The result is a dense channels-last tensor of the input's type. `weight` and
+    `bias` are (C,) tensors of one type, fp32 or the input's, so fp32 parameters serve 16-bit maps. Everything is
+    computed in fp32 and rounded once, at the end of the whole chain. `dropout_p`, `seed`, `offset` and `training` are
+    those of `dropout`, which gives the same mask for the same map. For the backward pass only the input and two
+    numbers per image and group are kept.
     """
     _require_values(input, "input")
     if input.dim() != 4:
