@@ -192,8 +192,9 @@ def _require_parameter(t: torch.Tensor, name: str, channels: int, input: torch.T
 
 
 def _group_norm_backward(ctx: Any, grad: torch.Tensor):
-    x, weight, bias, moments, _ = ctx.saved_tensors
+    x, weight, bias, moments, seed_tensor = ctx.saved_tensors
     cfg = _lib.GroupNormConfig.from_buffer_copy(ctx.cfg)   # two backward passes of one forward pass may run at once
+    cfg.seed_dev = _address(seed_tensor)   # hooks on saved tensors may have let the forward pass's own go
     grad, cfg.grad_image_stride, cfg.grad_pixel_stride = _channels_last(grad)
     need_x, need_weight, need_bias, _ = ctx.needs_input_grad
     new = torch.empty_like if x.numel() else torch.zeros_like

@@ -3,6 +3,7 @@ derives the tolerances)."""
 import numpy as np
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 from inpc_amd import _lib, dropout, fused_cauchy_loss, group_norm, rasterize_points, synthetic
 from tests import helpers as H
@@ -412,6 +413,36 @@ def test_a_training_step_from_points_to_loss(gpu):
     for got, ref in zip((grads[0][None], *grads[2:]), want):
         assert float((got.cpu().double() - ref).abs().max()) < 2000 * R.U * float(ref.abs().max())
     assert grads[1].shape == f.shape and bool(torch.isfinite(grads[1]).all()) and float(grads[1].abs().max()) > 0
+
+
+# ---- saved tensors that come back as others -------------------------------------------------------------------------
+
+SEEDED = {"group_norm": lambda t, seed: group_norm(t, 2, activation="silu", dropout_p=0.5, seed=seed, offset=3),
+          "dropout": lambda t, seed: dropout(t, 0.5, seed, offset=3)}
+
+
+def seeded_gradient(op, x, dy, seed, around=lambda f, t: f(t), before_backward=lambda: None):
+    """d(op(x) dy) / dx, where `around` calls the operator and `before_backward` comes between the two passes"""
+    xd = to_device(x).requires_grad_(True)
+    y = around(lambda t: SEEDED[op](t, seed()), xd)
+    before_backward()
+    y.backward(to_device(dy))
+    return xd.grad.cpu()
+
+
+@pytest.mark.parametrize("op", list(SEEDED))
+def test_checkpoint_of_a_call_whose_seed_tensor_is_let_go(gpu, op):
+    gen = torch.Generator().manual_seed(6)
+    x, dy = (torch.randn(2, 8, 5, 6, generator=gen) for _ in range(2))
+    kept = []
+
+    def refill():   # what the allocator hands out next lies where the seed was
+        kept.extend(torch.full((1,), k, dtype=torch.int64, device=H.DEVICE) for k in range(500))
+
+    want = seeded_gradient(op, x, dy, lambda: 1234567)
+    got = seeded_gradient(op, x, dy, lambda: torch.tensor([1234567], device=H.DEVICE),
+                          lambda f, t: checkpoint(f, t, use_reentrant=False), refill)
+    assert torch.equal(got, want)
 
 
 # ---- refusals ------------------------------------------------------------------------------------------------------

@@ -32,6 +32,8 @@ CASES = [
     ("test_group_norm_of_nothing", {}),
     ("test_norm_then_dropout_is_the_chain_of_both", {}),
     ("test_a_training_step_from_points_to_loss", {}),
+    ("test_checkpoint_of_a_call_whose_seed_tensor_is_let_go", dict(op="group_norm")),
+    ("test_checkpoint_of_a_call_whose_seed_tensor_is_let_go", dict(op="dropout")),
     ("test_refusals", {}),
 ]
 
