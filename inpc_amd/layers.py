@@ -76,9 +76,9 @@ def _dropout_call(x: torch.Tensor, p: float, seed: int, seed_tensor: torch.Tenso
 
 
 def _dropout_backward(ctx: Any, grad: torch.Tensor):
-    if ctx.random[2] is not None:
-        ctx.saved_tensors   # refuses a seed tensor that has changed
-    return _dropout_call(grad.contiguous(memory_format=ctx.order), *ctx.random), None, None
+    p, seed, offset = ctx.random
+    (seed_tensor,) = ctx.saved_tensors or (None,)   # torch refuses one that has changed; a hook's copy keeps its value
+    return _dropout_call(grad.contiguous(memory_format=ctx.order), p, seed, seed_tensor, offset), None, None
 
 
 # Under create_graph the result must refuse to be differentiated again; otherwise that wrapper's few microseconds are saved.
@@ -88,9 +88,10 @@ _dropout_backward_once = once_differentiable(_dropout_backward)
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, order: torch.memory_format, random: tuple) -> torch.Tensor:
-        ctx.order, ctx.random = order, random
-        if random[2] is not None:
-            ctx.save_for_backward(random[2])   # torch watches over it
+        p, seed, seed_tensor, offset = random
+        ctx.order, ctx.random = order, (p, seed, offset)
+        if seed_tensor is not None:
+            ctx.save_for_backward(seed_tensor)   # torch watches over it
         return _dropout_call(x, *random)
 
     @staticmethod

@@ -445,6 +445,20 @@ def test_checkpoint_of_a_call_whose_seed_tensor_is_let_go(gpu, op):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("op", list(SEEDED))
+def test_a_saved_copy_of_the_seed_outlives_a_refill(gpu, op):
+    gen = torch.Generator().manual_seed(7)
+    x, dy = (torch.randn(2, 8, 5, 6, generator=gen) for _ in range(2))
+    held = torch.tensor([77], device=H.DEVICE)
+
+    def copied(f, t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda saved: saved.clone(), lambda saved: saved):
+            return f(t)
+
+    want = seeded_gradient(op, x, dy, lambda: 77)
+    assert torch.equal(seeded_gradient(op, x, dy, lambda: held, copied, lambda: held.fill_(99)), want)
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
 def test_refusals(gpu):

@@ -34,6 +34,8 @@ CASES = [
     ("test_a_training_step_from_points_to_loss", {}),
     ("test_checkpoint_of_a_call_whose_seed_tensor_is_let_go", dict(op="group_norm")),
     ("test_checkpoint_of_a_call_whose_seed_tensor_is_let_go", dict(op="dropout")),
+    ("test_a_saved_copy_of_the_seed_outlives_a_refill", dict(op="group_norm")),
+    ("test_a_saved_copy_of_the_seed_outlives_a_refill", dict(op="dropout")),
     ("test_refusals", {}),
 ]
 
