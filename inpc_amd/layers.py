@@ -54,10 +54,17 @@ def _require_seed(seed: int | torch.Tensor | None, offset: int, device: torch.de
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
             raise RuntimeError("a seed tensor holds one Long on the device of the input")
-        return 0, seed, offset
+        return 0, seed.view(1), offset
     if seed is None or isinstance(seed, bool) or not isinstance(seed, int) or not 0 <= seed < 2**64:
         raise ValueError("dropout needs a seed: a whole number in [0, 2^64) or a tensor that holds one")
     return seed, None, offset
+
+
+def _require_unpacked(t: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype, grad: torch.Tensor) -> None:
+    """A hook on saved tensors gives back what it likes; the kernels go by the forward pass's sizes and types."""
+    if t is not None and (t.shape != shape or t.dtype != dtype or t.device != grad.device):
+        raise RuntimeError(f"a saved tensor of shape {tuple(shape)} and type {dtype} on {grad.device} was unpacked as {tuple(t.shape)}, "
+                           f"{t.dtype} on {t.device}")
 
 
 # ---- dropout -------------------------------------------------------------------------------------------------------
@@ -78,6 +85,7 @@ def _dropout_call(x: torch.Tensor, p: float, seed: int, seed_tensor: torch.Tenso
 def _dropout_backward(ctx: Any, grad: torch.Tensor):
     p, seed, offset = ctx.random
     (seed_tensor,) = ctx.saved_tensors or (None,)   # torch refuses one that has changed; a hook's copy keeps its value
+    _require_unpacked(seed_tensor, (1,), torch.int64, grad)
     return _dropout_call(grad.contiguous(memory_format=ctx.order), p, seed, seed_tensor, offset), None, None
 
 
@@ -195,7 +203,15 @@ def _require_parameter(t: torch.Tensor, name: str, channels: int, input: torch.T
 def _group_norm_backward(ctx: Any, grad: torch.Tensor):
     x, weight, bias, moments, seed_tensor = ctx.saved_tensors
     cfg = _lib.GroupNormConfig.from_buffer_copy(ctx.cfg)   # two backward passes of one forward pass may run at once
-    cfg.seed_dev = _address(seed_tensor)   # hooks on saved tensors may have let the forward pass's own go
+    # Hooks on saved tensors may give back others than the forward pass's, which lie elsewhere and with other strides.
+    _require_unpacked(x, grad.shape, grad.dtype, grad)
+    _require_unpacked(weight, (cfg.channels,), ctx.param_dtype, grad)
+    _require_unpacked(bias, (cfg.channels,), ctx.param_dtype, grad)
+    _require_unpacked(moments, (2 * cfg.n_images * cfg.groups,), torch.float32, grad)
+    _require_unpacked(seed_tensor, (1,), torch.int64, grad)
+    x, cfg.input_image_stride, cfg.input_pixel_stride = _channels_last(x)
+    weight, bias, moments = (t if t is None else t.contiguous() for t in (weight, bias, moments))
+    cfg.seed_dev = _address(seed_tensor)
     grad, cfg.grad_image_stride, cfg.grad_pixel_stride = _channels_last(grad)
     need_x, need_weight, need_bias, _ = ctx.needs_input_grad
     new = torch.empty_like if x.numel() else torch.zeros_like
@@ -216,6 +232,7 @@ class _GroupNorm(torch.autograd.Function):
     def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, options: tuple) -> torch.Tensor:
         y, x, moments, ctx.cfg = _group_norm_call(x, weight, bias, *options)
         ctx.save_for_backward(x, weight, bias, moments, options[5])   # the last: a seed on the GPU, which torch watches over
+        ctx.param_dtype = next((t.dtype for t in (weight, bias) if t is not None), None)
         return y
 
     @staticmethod

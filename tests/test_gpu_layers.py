@@ -459,6 +459,52 @@ def test_a_saved_copy_of_the_seed_outlives_a_refill(gpu, op):
     assert torch.equal(seeded_gradient(op, x, dy, lambda: held, copied, lambda: held.fill_(99)), want)
 
 
+def test_saved_tensors_that_come_back_with_other_strides(gpu):
+    """Hooks that keep values alone (as copies into pinned memory do): the input comes back row-major, and a slice of a wider map
+    as a map of its own; parameters come back strided."""
+    x, weight, bias, dy = make_case(2, 16, 9, 10, "fp32", 3)
+    held = torch.tensor([4], device=H.DEVICE)
+
+    def gradients(map_on_device, hooked):
+        leaves = [t.requires_grad_(True) for t in (map_on_device(x), to_device(weight), to_device(bias))]
+        pack = lambda t: t.clone(memory_format=torch.contiguous_format)  # noqa: E731
+        unpack = lambda t: torch.stack((t, t), 1)[:, 0] if t.dim() == 1 else t  # noqa: E731
+        with torch.autograd.graph.saved_tensors_hooks(*((pack, unpack) if hooked else (lambda t: t, lambda t: t))):
+            y = group_norm(leaves[0], 4, *leaves[1:], activation="silu", dropout_p=0.2, seed=held)
+        return torch.autograd.grad(y, leaves, to_device(dy))
+
+    for map_on_device in (to_device, lambda t: to_device(torch.cat((t, t, t), 1))[:, 16:32], lambda t: to_device(t).contiguous()):
+        want = gradients(map_on_device, False)
+        for got, ref in zip(gradients(map_on_device, True), want):
+            assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("which", ["input", "weight", "bias", "moments", "seed"])
+def test_saved_tensors_that_come_back_as_something_else_are_refused(gpu, which):
+    # in the order in which the operator saves them; sizes, types and places that the kernels would read past
+    position = ["input", "weight", "bias", "moments", "seed"].index(which)
+    x, weight, bias, dy = make_case(2, 8, 5, 6, "fp32", 3)
+    held = torch.tensor([4], device=H.DEVICE)
+    for changed in (lambda t: t[:0], lambda t: t.to(torch.bfloat16 if t.is_floating_point() else torch.int32), lambda t: t.to("meta")):
+        packed = []
+
+        def pack(t):
+            packed.append(t)
+            return len(packed) - 1
+
+        leaves = [to_device(t).requires_grad_(True) for t in (x, weight, bias)]
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda i: changed(packed[i]) if i == position else packed[i]):
+            y = group_norm(leaves[0], 2, *leaves[1:], dropout_p=0.5, seed=held)
+        assert len(packed) == 5
+        with pytest.raises(RuntimeError, match="unpacked"):
+            torch.autograd.grad(y, leaves, to_device(dy))
+        if which == "seed":
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, changed):
+                y = dropout(leaves[0], 0.5, held)
+            with pytest.raises(RuntimeError, match="unpacked"):
+                torch.autograd.grad(y, leaves[0], to_device(dy))
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
 def test_refusals(gpu):

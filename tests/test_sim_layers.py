@@ -36,6 +36,9 @@ CASES = [
     ("test_checkpoint_of_a_call_whose_seed_tensor_is_let_go", dict(op="dropout")),
     ("test_a_saved_copy_of_the_seed_outlives_a_refill", dict(op="group_norm")),
     ("test_a_saved_copy_of_the_seed_outlives_a_refill", dict(op="dropout")),
+    ("test_saved_tensors_that_come_back_with_other_strides", {}),
+    *(("test_saved_tensors_that_come_back_as_something_else_are_refused", dict(which=which))
+      for which in ("input", "weight", "bias", "moments", "seed")),
     ("test_refusals", {}),
 ]
 
