@@ -3,6 +3,7 @@ derives the tolerances)."""
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from inpc_amd import _lib, dropout, fused_cauchy_loss, group_norm, rasterize_points, synthetic
@@ -555,6 +556,26 @@ def test_refusals(gpu):
         (g,) = torch.autograd.grad(y.square().sum(), xg, create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(g.sum(), xg)
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_is_refused(gpu, grad_mode):
+    x, weight, bias, dy = (to_device(t) for t in make_case(1, 8, 4, 5, "fp32", 13))
+    xg = x.clone().requires_grad_(grad_mode)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: dropout(dual(x), 0.5, 1), lambda: group_norm(dual(x), 2), lambda: dropout(dual(xg), 0.5, 1),
+                     lambda: group_norm(x, 2, dual(weight), bias), lambda: group_norm(x, 2, weight, dual(bias)),
+                     lambda: group_norm(xg, 2, dual(weight), bias)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert forward_ad.unpack_dual(dropout(dual(x), 0.0, None)).tangent is not None   # the input itself
+        # no tangent, nothing to lose
+        group_norm(x, 2, weight, bias), dropout(x, 0.5, 1)
+        if grad_mode:   # forward over reverse
+            for y in (group_norm(xg, 2, weight, bias), dropout(xg, 0.5, 1)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch.autograd.grad(y, xg, dual(dy))
 
 
 # ---- on the device alone: graphs, streams, sizes -------------------------------------------------------------------

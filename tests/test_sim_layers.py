@@ -40,6 +40,8 @@ CASES = [
     *(("test_saved_tensors_that_come_back_as_something_else_are_refused", dict(which=which))
       for which in ("input", "weight", "bias", "moments", "seed")),
     ("test_refusals", {}),
+    ("test_forward_mode_is_refused", dict(grad_mode=True)),
+    ("test_forward_mode_is_refused", dict(grad_mode=False)),
 ]
 
 
