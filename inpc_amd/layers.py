@@ -34,18 +34,24 @@ def _address(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def _require_plain_call(*tensors: torch.Tensor | None) -> None:
+    """Refuses what torch does around its own operators and would leave a kernel out of. The kernels compute no forward-mode
+    derivatives, and what they write carries none; a recorded call would replay the allocation of the result alone."""
+    if forward_ad._current_level >= 0:   # no dual tensors outside of a level: that alone is asked in most calls (0.07 us)
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise RuntimeError("group_norm and dropout have no forward-mode derivative")
+    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+        raise RuntimeError("group_norm and dropout cannot be recorded by torch.jit.trace or make_fx; capture a CUDA graph instead")
+
+
 def _require_values(t: torch.Tensor, name: str) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"expected {name} to be a tensor on the GPU")
     if t.dtype not in _DTYPES:
         raise RuntimeError(f"expected {name} of scalar type Float, Half or BFloat16, got {t.dtype}")
-
-
-def _require_no_tangent(*tensors: torch.Tensor | None) -> None:
-    """The kernels compute no forward-mode derivatives, and what they write carries none."""
-    if forward_ad._current_level >= 0:   # no dual tensors outside of a level: that alone is asked in most calls (0.07 us)
-        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-            raise RuntimeError("group_norm and dropout have no forward-mode derivative")
 
 
 def _require_probability(p: float, name: str) -> float:
@@ -91,7 +97,7 @@ def _dropout_call(x: torch.Tensor, p: float, seed: int, seed_tensor: torch.Tenso
 
 
 def _dropout_backward(ctx: Any, grad: torch.Tensor):
-    _require_no_tangent(grad)
+    _require_plain_call(grad)
     p, seed, offset = ctx.random
     (seed_tensor,) = ctx.saved_tensors or (None,)   # torch refuses one that has changed; a hook's copy keeps its value
     _require_unpacked(seed_tensor, (1,), torch.int64, grad)
@@ -132,7 +138,7 @@ def dropout(input: torch.Tensor, p: float, seed: int | torch.Tensor | None, offs
     p = _require_probability(p, "p")
     if not training or p == 0.0:
         return input
-    _require_no_tangent(input)
+    _require_plain_call(input)
     random = (p, *_require_seed(seed, offset, input.device))
     order = _memory_format(input)
     input = input.contiguous(memory_format=order)
@@ -212,7 +218,7 @@ def _require_parameter(t: torch.Tensor, name: str, channels: int, input: torch.T
 
 def _group_norm_backward(ctx: Any, grad: torch.Tensor):
     x, weight, bias, moments, seed_tensor = ctx.saved_tensors
-    _require_no_tangent(grad, x, weight, bias)
+    _require_plain_call(grad, x, weight, bias)
     cfg = _lib.GroupNormConfig.from_buffer_copy(ctx.cfg)   # two backward passes of one forward pass may run at once
     # Hooks on saved tensors may give back others than the forward pass's, which lie elsewhere and with other strides.
     _require_unpacked(x, grad.shape, grad.dtype, grad)
@@ -282,7 +288,7 @@ def group_norm(input: torch.Tensor, num_groups: int, weight: torch.Tensor | None
         bias = _require_parameter(bias, "bias", channels, input)
         if weight is not None and weight.dtype != bias.dtype:
             raise RuntimeError("weight and bias have one scalar type, Float or that of the input")
-    _require_no_tangent(input, weight, bias)
+    _require_plain_call(input, weight, bias)
     p = _require_probability(dropout_p, "dropout_p") if training else 0.0
     seed, seed_tensor, offset = _require_seed(seed, offset, input.device) if p > 0.0 else (0, None, 0)
     options = num_groups, float(eps), _ACTIVATIONS[activation], p, seed, seed_tensor, offset

@@ -578,6 +578,23 @@ def test_forward_mode_is_refused(gpu, grad_mode):
                     torch.autograd.grad(y, xg, dual(dy))
 
 
+@pytest.mark.parametrize("requires_grad", [True, False])
+def test_recording_is_refused(gpu, requires_grad):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.randn(1, 4, 3, 5, device=H.DEVICE, requires_grad=requires_grad)
+    for call in (lambda t: dropout(t, 0.5, 1), lambda t: group_norm(t, 2)):
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(call)(x)
+        with pytest.raises(RuntimeError, match="recorded"):
+            torch.jit.trace(call, x, check_trace=False)
+        y = call(x)
+        if requires_grad:   # the backward pass alone
+            with pytest.raises(RuntimeError, match="recorded"):
+                make_fx(lambda dy: torch.autograd.grad(y, x, dy))(torch.ones_like(y))
+    assert torch.equal(torch.jit.trace(lambda t: 2 * dropout(t, 0.5, None, training=False), x)(x), 2 * x)
+
+
 # ---- on the device alone: graphs, streams, sizes -------------------------------------------------------------------
 
 @pytest.mark.real_gpu

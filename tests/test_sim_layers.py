@@ -42,6 +42,8 @@ CASES = [
     ("test_refusals", {}),
     ("test_forward_mode_is_refused", dict(grad_mode=True)),
     ("test_forward_mode_is_refused", dict(grad_mode=False)),
+    ("test_recording_is_refused", dict(requires_grad=True)),
+    ("test_recording_is_refused", dict(requires_grad=False)),
 ]
 
 
