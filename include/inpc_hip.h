@@ -616,7 +616,8 @@ int inpc_group_norm_forward(const inpc_group_norm_config* cfg, const void* input
 /* Gradients of the same (the layers of Modules/UNet.py:1-200): grad_input dense like the output, grad_weight and
  * grad_bias (channels,) of param_dtype; any of the three may be NULL. `moments` is what the forward call wrote;
  * seed (or what seed_dev points to) and offset have to be those of the forward call: the mask is
- * computed again. */
+ * computed again. A map without values (n_images or n_pixels 0) gives zeros in grad_weight and grad_bias; its forward call
+ * writes nothing, moments included. */
 int inpc_group_norm_backward(const inpc_group_norm_config* cfg, const void* grad_output,
                              const void* input, const void* weight, const void* bias,
                              const float* moments, void* grad_input, void* grad_weight,

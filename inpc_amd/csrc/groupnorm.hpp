@@ -1014,6 +1014,15 @@ int backward_split(const inpc_group_norm_config& cfg, const void* x, const void*
     return INPC_OK;
 }
 
+// Of a map without values: the parameters' gradients are sums over nothing.
+inline int backward_of_nothing(const inpc_group_norm_config& cfg, void* dweight, void* dbias, hipStream_t stream) {
+    const Shape s = base_shape(cfg);
+    if (dweight || dbias)
+        INPC_LAUNCH("group_norm_parameter_gradients", k_parameter_gradients, dim3(div_up(s.channels, kParameterColumns)), dim3(kThreads),
+                    stream, (const float2*)nullptr, 0u, dweight, dbias, s);
+    return INPC_OK;
+}
+
 // Calls f<dtype, vector width>(args...).
 #define INPC_NORM_DISPATCH(f, dtype, v, ...)                                                              \
     ((dtype) == INPC_DTYPE_F32   ? ((v) == 4 ? f<INPC_DTYPE_F32, 4>(__VA_ARGS__)                           \

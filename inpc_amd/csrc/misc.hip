@@ -190,7 +190,8 @@ int inpc_group_norm_backward(const inpc_group_norm_config* cfg, const void* grad
                              void* workspace, size_t workspace_bytes, void* stream) {
     using namespace inpc;
     if (const int rc = norm::check_config(cfg, "group_norm_backward")) return rc;
-    if (cfg->n_images == 0 || cfg->n_pixels == 0 || !(grad_input || grad_weight || grad_bias)) return INPC_OK;
+    if (!(grad_input || grad_weight || grad_bias)) return INPC_OK;
+    if (cfg->n_images == 0 || cfg->n_pixels == 0) return norm::backward_of_nothing(*cfg, grad_weight, grad_bias, (hipStream_t)stream);
     if (!grad_output || !input || !moments) return fail(INPC_E_INVALID_ARGUMENT, "group_norm_backward: null pointer");
     if (const int rc = norm::check_workspace(*cfg, true, workspace, workspace_bytes, "group_norm_backward")) return rc;
     return norm::backward(*cfg, input, grad_output, (const float2*)moments, weight, bias, grad_input, grad_weight, grad_bias,

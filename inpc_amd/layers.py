@@ -231,10 +231,9 @@ def _group_norm_backward(ctx: Any, grad: torch.Tensor):
     cfg.seed_dev = _address(seed_tensor)
     grad, cfg.grad_image_stride, cfg.grad_pixel_stride = _channels_last(grad)
     need_x, need_weight, need_bias, _ = ctx.needs_input_grad
-    new = torch.empty_like if x.numel() else torch.zeros_like
     dx = _dense(x) if need_x else None
-    dweight = new(weight) if need_weight else None
-    dbias = new(bias) if need_bias else None
+    dweight = torch.empty_like(weight) if need_weight else None
+    dbias = torch.empty_like(bias) if need_bias else None
     workspace, size = _workspace(cfg, 1, x.device)
     _run("inpc_group_norm_backward", x, C.byref(cfg), grad.data_ptr(), x.data_ptr(), _address(weight), _address(bias),
          moments.data_ptr(), _address(dx), _address(dweight), _address(dbias), _address(workspace), size)

@@ -366,6 +366,26 @@ def test_group_norm_of_nothing(gpu):
         assert x.grad.shape == size and torch.equal(w.grad.cpu(), torch.zeros(4))
 
 
+@pytest.mark.parametrize("param", ["fp32", "bf16"])
+@pytest.mark.parametrize("size", [dict(n_images=0, n_pixels=9), dict(n_images=2, n_pixels=0)], ids=["no image", "no pixel"])
+def test_gradients_of_nothing_through_the_c_abi(gpu, size, param):
+    """The parameters' gradients are sums over nothing: zeros, in buffers that held something else."""
+    channels = 70
+    cfg = _lib.GroupNormConfig(**size, channels=channels, groups=7, dtype=_lib.DTYPE_BF16,
+                               param_dtype=_lib.DTYPE_F32 if param == "fp32" else _lib.DTYPE_BF16, activation=0, eps=1e-5,
+                               input_image_stride=0, input_pixel_stride=channels, grad_image_stride=0, grad_pixel_stride=channels)
+    for wanted in ((True, True), (True, False), (False, True)):
+        grads = [torch.full((channels + 1,), 7.0, dtype=DTYPES[param], device=H.DEVICE) for _ in range(2)]
+        args = [_lib.ptr(g) if want else None for g, want in zip(grads, wanted)]
+        _lib.check(_lib.lib().inpc_group_norm_backward(cfg, None, None, None, None, None, None, *args, None, 0, H.stream()),
+                   "inpc_group_norm_backward")
+        for g, want in zip(grads, wanted):
+            expected = torch.full((channels + 1,), 7.0, dtype=DTYPES[param])
+            if want:
+                expected[:channels] = 0
+            assert torch.equal(g.cpu(), expected)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 def test_norm_then_dropout_is_the_chain_of_both(gpu):

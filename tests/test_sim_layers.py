@@ -30,6 +30,8 @@ CASES = [
     ("test_group_norm_gradient_against_differences", {}),
     ("test_group_norm_keeps_what_is_not_finite_inside_its_group", dict(size=(90, 101))),
     ("test_group_norm_of_nothing", {}),
+    ("test_gradients_of_nothing_through_the_c_abi", dict(size=dict(n_images=0, n_pixels=9), param="fp32")),
+    ("test_gradients_of_nothing_through_the_c_abi", dict(size=dict(n_images=2, n_pixels=0), param="bf16")),
     ("test_norm_then_dropout_is_the_chain_of_both", {}),
     ("test_a_training_step_from_points_to_loss", {}),
     ("test_checkpoint_of_a_call_whose_seed_tensor_is_let_go", dict(op="group_norm")),
