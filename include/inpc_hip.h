@@ -592,7 +592,7 @@ typedef struct inpc_group_norm_config {
     float eps;
     uint64_t input_image_stride, input_pixel_stride;
     uint64_t grad_image_stride, grad_pixel_stride;
-    double dropout_p;            /* 0: no dropout. The rest as for inpc_dropout                   */
+    double dropout_p;            /* 0: no dropout, seed_dev is not read. Else as for inpc_dropout  */
     uint64_t seed;
     const uint64_t* seed_dev;
     uint64_t offset;

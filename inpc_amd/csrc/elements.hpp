@@ -148,7 +148,7 @@ __device__ __forceinline__ void store_element(void* base, int32_t dtype, size_t 
 // twenty 32x32->64-bit products, the generator's whole cost at quarter rate, per vector instead of per half.
 struct Dropout {
     uint64_t seed, offset;
-    const uint64_t* seed_dev;   // where not null: the seed's place in device memory
+    const uint64_t* seed_dev;   // where not null: the seed's place in device memory; null where nothing is dropped, whatever the caller's
     uint32_t upper, lower;      // T = upper * 2^16 + lower, upper <= 2^16
     float scale;                // 1 / (1 - p); 0 where everything is dropped
     uint32_t on;
@@ -156,7 +156,7 @@ struct Dropout {
 
 inline Dropout make_dropout(double p, uint64_t seed, const uint64_t* seed_dev, uint64_t offset) {
     const uint64_t threshold = (uint64_t)std::nearbyint(p * 4294967296.0);
-    return Dropout{seed, offset, seed_dev, (uint32_t)(threshold >> 16), (uint32_t)(threshold & 0xFFFFu),
+    return Dropout{seed, offset, p > 0.0 ? seed_dev : nullptr, (uint32_t)(threshold >> 16), (uint32_t)(threshold & 0xFFFFu),
                    p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f, p > 0.0 ? 1u : 0u};
 }
 

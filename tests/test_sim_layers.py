@@ -10,6 +10,9 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
+
+from inpc_amd import _lib
 
 CASES = [
     ("test_dropout_is_its_definition_bit_for_bit", dict(count=10007, dtype="bf16")),
@@ -61,6 +64,31 @@ def test_on_the_simulator(sim, case):
     assert set(inspect.signature(function).parameters) == {"gpu", *kwargs}
     assert "real_gpu" not in [m.name for m in getattr(function, "pytestmark", [])]
     function(gpu=sim, **kwargs)
+
+
+def test_the_seed_of_a_call_without_dropout_is_not_read(sim):
+    """Its address may be anything: none of these runs on a device, where reading it would fault."""
+    gen = torch.Generator().manual_seed(1)
+    nowhere = 8
+    for pixels in (16, 9000):   # either form
+        x, dy = (torch.randn(pixels, 8, generator=gen) for _ in range(2))
+        results = []
+        for seed_dev in (None, nowhere):
+            cfg = _lib.GroupNormConfig(1, pixels, 8, 2, _lib.DTYPE_F32, _lib.DTYPE_F32, 2, 1e-5, pixels * 8, 8, pixels * 8, 8, 0.0, 5,
+                                       seed_dev, 0)
+            y, dx, dw, moments = torch.empty_like(x), torch.empty_like(x), torch.empty(8), torch.empty(4)
+            lib = _lib.lib()
+            workspace = [torch.empty(lib.inpc_group_norm_workspace_bytes(cfg, backward) + 16, dtype=torch.uint8) for backward in (0, 1)]
+            _lib.check(lib.inpc_group_norm_forward(cfg, _lib.ptr(x), None, None, _lib.ptr(y), _lib.ptr(moments), _lib.ptr(workspace[0]),
+                                                   workspace[0].numel(), None), "inpc_group_norm_forward")
+            _lib.check(lib.inpc_group_norm_backward(cfg, _lib.ptr(dy), _lib.ptr(x), None, None, _lib.ptr(moments), _lib.ptr(dx),
+                                                    _lib.ptr(dw), None, _lib.ptr(workspace[1]), workspace[1].numel(), None),
+                       "inpc_group_norm_backward")
+            copied = torch.empty_like(x)
+            _lib.check(lib.inpc_dropout(_lib.ptr(x), _lib.ptr(copied), x.numel(), _lib.DTYPE_F32, 0.0, 5, seed_dev, 0, None), "inpc_dropout")
+            assert torch.equal(copied, x)
+            results.append((y, dx, dw, moments))
+        assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
 @pytest.mark.parametrize("order", ["reverse", "shuffle"])
