@@ -274,6 +274,20 @@ def test_group_norm_of_values_far_from_zero(gpu):
           torch.randn(1, 4, 5, 5, generator=gen), 2)
 
 
+def outlier_in_front(n, c, h, w, dtype, seed):
+    """Every image's first value makes up most of its variance: the worst pivot there is."""
+    x, _, _, dy = make_case(n, c, h, w, dtype, seed, mean=0.0, weighted=False)
+    x[:, 0, 0, 0] = 3e4
+    return x, dy
+
+
+@pytest.mark.parametrize("shape", [(1, 2056, 64, 64, 1, "fp32"), (1, 515, 64, 64, 1, "fp16"), (256, 1, 256, 256, 1, "fp16")], ids=str)
+def test_group_norm_of_an_outlier_in_front_of_many_values(gpu, shape):
+    *size, groups, dtype = shape
+    x, dy = outlier_in_front(*size, dtype, 23)
+    check(x, None, None, dy, groups)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_group_norm_layouts(gpu, dtype):
     gen = torch.Generator().manual_seed(12)
@@ -723,6 +737,17 @@ def test_more_than_two_to_the_32_values(gpu):
         ref = R.activation(z, "silu") * keep.permute(2, 0, 1) * 2.0
         # moments of 16.8 million pixels: a chain of up to 2^12 roundings, and half a step of bf16
         R.assert_within(y[-1, 16 * group:16 * group + 16, -rows:], ref, 4096 * R.U * (z.abs() + 1) + 2.0**-8 * ref.abs(), "y")
+
+
+@pytest.mark.real_gpu
+def test_an_outlier_in_front_of_long_runs(gpu):
+    """512 images, so that a block has a whole one and a thread 512 vectors (2.1 GB): two of them against the reference."""
+    x = torch.randn(512, 64, 128, 128, generator=torch.Generator(device=gpu).manual_seed(2), device=gpu).permute(0, 3, 1, 2)
+    x[:, ::4, 0, 0] = 3e4
+    y = group_norm(x, 32)
+    for image in (0, 511):
+        ref = R.GroupNorm(x[image:image + 1].cpu(), 32, None, None, 1e-5, "none")
+        R.assert_within(y[image:image + 1], ref.y, ref.y_bound, "y")
 
 
 @pytest.mark.real_gpu

@@ -30,6 +30,9 @@ CASES = [
     ("test_group_norm_activation_and_dropout", dict(act="silu", p=0.35, dtype="bf16")),
     ("test_group_norm_layouts", dict(dtype="bf16")),
     ("test_group_norm_of_values_far_from_zero", {}),
+    ("test_group_norm_of_an_outlier_in_front_of_many_values", dict(shape=(1, 2056, 64, 64, 1, "fp32"))),
+    ("test_group_norm_of_an_outlier_in_front_of_many_values", dict(shape=(1, 515, 64, 64, 1, "fp16"))),
+    ("test_group_norm_of_an_outlier_in_front_of_many_values", dict(shape=(256, 1, 256, 256, 1, "fp16"))),
     ("test_group_norm_gradient_against_differences", {}),
     ("test_group_norm_keeps_what_is_not_finite_inside_its_group", dict(size=(90, 101))),
     ("test_group_norm_of_nothing", {}),
