@@ -6,8 +6,8 @@
 //   dx = (weight * dz - A - xhat * B) / sqrt(var + eps), A and B the group's means of weight * dz and weight * dz * xhat
 //
 // Two forms. "single": a block per (image, group) does everything in one launch, for small maps, whose launches and latencies
-// cost more than their bytes. "split": a block per run of pixels (a slab) of an image, all channels wide, so that it reads
-// whole runs of memory; one launch writes each slab's sums, the next adds them up at the start of every block (or a
+// cost more than their bytes. "split": a block per run of pixels (a slab) of an image and tile of its channels, as wide as a block can
+// be, so that it reads whole runs of memory; one launch writes each slab's sums, the next adds them up at the start of every block (or a
 // launch in between does) and applies. In both a thread keeps one vector of channels (16 bytes where channel counts, strides
 // and pointers allow). Sums are fp32 in an order that depends on sizes and alignments alone (no atomics); deviations are
 // taken from a value of the data, so that nothing cancels however far the values are from 0.
@@ -53,6 +53,8 @@ struct Shape {
     uint32_t n, pixels, channels, groups, per_group;
     uint32_t columns, rows;      // threads of a block: vectors side by side, pixels at once
     uint32_t tiles, tile_groups; // split form: tiles of channels, and whole groups in each (fewer in the last)
+    uint32_t parts;              // ... or, where a group is too wide for a block, this many tiles to each group (tile_groups is 1)
+    uint32_t tile_channels;      // ... channels of a tile (fewer in the last)
     uint32_t slabs, slab_pixels; // ... and runs of pixels of each tile of an image
     int32_t activation, param_dtype;
     float eps;
@@ -503,9 +505,10 @@ __global__ void __launch_bounds__(kThreads) k_parameter_gradients(const float2* 
 }
 
 // ---- the split form --------------------------------------------------------------------------------------------------
-// What a block works on: a slab of pixels and a tile of channels (whole groups) of one image
+// What a block works on: a slab of pixels and a tile of channels (whole groups, or a part of one) of one image
 struct Place {
-    uint32_t image, tile, channel;   // `channel`: the tile's first
+    uint32_t image, tile, part, channel, width;   // `channel`: the tile's first; `width`: its channels
+    uint32_t group, groups, group_width;          // its first group, its groups, and the channels of each in the tile
     uint32_t slab, begin, size;
 };
 
@@ -514,7 +517,19 @@ __device__ __forceinline__ Place place_of(const Shape& s, uint32_t block) {
     const uint32_t rest = block / s.slabs;
     p.tile = rest % s.tiles;
     p.image = rest / s.tiles;
-    p.channel = p.tile * s.tile_groups * s.per_group;
+    if (s.parts == 1) {
+        p.part = 0;
+        p.group = p.tile * s.tile_groups;
+        p.groups = min(s.tile_groups, s.groups - p.group);
+        p.group_width = s.per_group;
+    } else {
+        p.part = p.tile % s.parts;
+        p.group = p.tile / s.parts;
+        p.groups = 1;
+        p.group_width = min(s.tile_channels, s.per_group - p.part * s.tile_channels);
+    }
+    p.channel = p.group * s.per_group + p.part * s.tile_channels;
+    p.width = p.groups * p.group_width;
     p.slab = block % s.slabs;
     p.begin = p.slab * s.slab_pixels;
     p.size = min(s.slab_pixels, s.pixels - p.begin);
@@ -531,11 +546,7 @@ __device__ __forceinline__ Numbers numbers_at(const Place& p, const Shape& s) {
     return numbers_of<V>(((uint64_t)p.image * s.pixels + p.begin) * s.channels + p.channel, s);
 }
 
-__device__ __forceinline__ uint32_t groups_of_tile(const Shape& s, uint32_t tile) {
-    return min(s.tile_groups, s.groups - tile * s.tile_groups);
-}
-
-// Slab sums lie [image][tile][group of the tile][slab]
+// Slab sums lie [image][tile][group of the tile][slab]: those of a group follow each other, also of one in parts
 __device__ __forceinline__ size_t sums_at(const Shape& s, const Place& p, uint32_t group) {
     return ((size_t)(p.image * s.tiles + p.tile) * s.tile_groups + group) * s.slabs;
 }
@@ -543,7 +554,7 @@ __device__ __forceinline__ size_t sums_at(const Shape& s, const Place& p, uint32
 // The calling thread's row in its block; a row of no slab where it has none or its channels are behind the last
 __device__ __forceinline__ uint32_t thread_row(const Shape& s, const Place& p, uint32_t vector) {
     const uint32_t row = threadIdx.x / s.columns;
-    return row < s.rows && p.channel + threadIdx.x % s.columns * vector < s.channels ? row : 0xFFFFFFFFu;
+    return row < s.rows && threadIdx.x % s.columns * vector < p.width ? row : 0xFFFFFFFFu;
 }
 
 // Sums over the slots of each group of a tile: values[row * width + slot], `per_group` neighbouring slots of all rows to a group.
@@ -581,10 +592,10 @@ __global__ void __launch_bounds__(kThreads) k_moments(const void* __restrict__ x
     });
     sums.join();
     // the group's mean, then everybody's deviations from it
-    const uint32_t groups = groups_of_tile(s, p.tile), width = s.columns * Q, slots = s.per_group / W;
+    const uint32_t groups = p.groups, width = s.columns * Q, slots = p.group_width / W;
     const uint32_t slot = threadIdx.x % s.columns * Q, at = threadIdx.x / s.columns * width + slot;
     const bool in_block = threadIdx.x / s.columns < s.rows;
-    const float in_group = (float)p.size * (float)s.per_group;
+    const float in_group = (float)p.size * (float)p.group_width;
     if (in_block)
 #pragma unroll
         for (int q = 0; q < Q; ++q) lds[at + q] = sums.sum(q);
@@ -593,7 +604,7 @@ __global__ void __launch_bounds__(kThreads) k_moments(const void* __restrict__ x
     if (in_block)
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
-            // the slots of a last tile's missing groups are nobody's
+            // the slots of a last tile's missing groups, or of a last part's missing channels, are nobody's
             const float of_group = (slot + q) / slots < groups ? group[(slot + q) / slots] / in_group : 0.0f;
             lds[at + q] = sums.deviations(q, of_group);
         }
@@ -603,21 +614,30 @@ __global__ void __launch_bounds__(kThreads) k_moments(const void* __restrict__ x
         partial[sums_at(s, p, threadIdx.x) + p.slab] = make_float2(group[threadIdx.x] / in_group, squares[threadIdx.x]);
 }
 
-// A group's moments from its slabs', by a power of two of lanes, in all of them: a lane's slabs with the first one's mean as the
-// pivot, then the lanes' deviations from the mean of all. `mine` is null for lanes of no group.
+// A group's moments from its slabs' (of all its parts), by a power of two of lanes, in all of them: a lane's slabs with the first
+// one's mean as the pivot, then the lanes' deviations from the mean of all. `mine` is null for lanes of no group.
 __device__ __forceinline__ float2 fold_moments(const float2* mine, const Shape& s, uint32_t lane, uint32_t lanes) {
     const float count = (float)s.pixels * (float)s.per_group, of_slab = (float)s.slab_pixels * (float)s.per_group;
-    const float of_last = (float)(s.pixels - (s.slabs - 1) * s.slab_pixels) * (float)s.per_group;
+    const uint32_t last_pixels = s.pixels - (s.slabs - 1) * s.slab_pixels, entries = s.parts * s.slabs;
+    const float of_last = (float)last_pixels * (float)s.per_group;
     float n = 0.0f, pivot = 0.0f, s1 = 0.0f, s2 = 0.0f;
-    if (mine && lane < s.slabs) {
+    const auto add = [&](const float2& v, float weight) {
+        const float d = v.x - pivot;
+        n += weight;
+        s1 = fmaf(weight, d, s1);
+        s2 += fmaf(weight * d, d, v.y);
+    };
+    if (mine && lane < entries) {
         pivot = mine[lane].x;
+        if (s.parts == 1) {
 #pragma unroll 8
-        for (uint32_t slab = lane; slab < s.slabs; slab += lanes) {
-            const float2 v = mine[slab];
-            const float weight = slab + 1 < s.slabs ? of_slab : of_last, d = v.x - pivot;
-            n += weight;
-            s1 = fmaf(weight, d, s1);
-            s2 += fmaf(weight * d, d, v.y);
+            for (uint32_t slab = lane; slab < s.slabs; slab += lanes) add(mine[slab], slab + 1 < s.slabs ? of_slab : of_last);
+        } else {
+            for (uint32_t i = lane; i < entries; i += lanes) {
+                const uint32_t part = i / s.slabs, slab = i % s.slabs;
+                add(mine[i], (float)(slab + 1 < s.slabs ? s.slab_pixels : last_pixels) *
+                                 (float)min(s.tile_channels, s.per_group - part * s.tile_channels));
+            }
         }
     }
     const float share = n > 0.0f ? s1 / n : 0.0f;
@@ -631,9 +651,9 @@ __device__ __forceinline__ float2 fold_gradients(const float2* mine, const Shape
     float a = 0.0f, b = 0.0f;
     if (mine)
 #pragma unroll 8
-        for (uint32_t slab = lane; slab < s.slabs; slab += lanes) {
-            a += mine[slab].x;
-            b += mine[slab].y;
+        for (uint32_t i = lane; i < s.parts * s.slabs; i += lanes) {
+            a += mine[i].x;
+            b += mine[i].y;
         }
     const float count = (float)s.pixels * (float)s.per_group;
     return make_float2(lanes_sum(a, lanes) / count, lanes_sum(b, lanes) / count);
@@ -642,8 +662,9 @@ __device__ __forceinline__ float2 fold_gradients(const float2* mine, const Shape
 // Of one tile of an image, into LDS: by every block of the launch that needs them where they are few ...
 template <typename F>
 __device__ __forceinline__ void fold_tile(const float2* partial, const Shape& s, const Place& p, float2* folded, F fold) {
-    const uint32_t groups = groups_of_tile(s, p.tile), lanes = lanes_for(groups), lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
-    const float2 m = fold(group < groups ? partial + sums_at(s, p, group) : nullptr, s, lane, lanes);
+    const uint32_t groups = p.groups, lanes = lanes_for(groups), lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+    const float2* first = partial + sums_at(s, p, 0) - (size_t)p.part * s.slabs;
+    const float2 m = fold(group < groups ? first + (size_t)group * s.slabs : nullptr, s, lane, lanes);
     if (lane == 0 && group < groups) folded[group] = m;
     __syncthreads();
 }
@@ -652,7 +673,7 @@ __device__ __forceinline__ void fold_tile(const float2* partial, const Shape& s,
 __device__ __forceinline__ const float2* sums_of_wave(const float2* partial, const Shape& s, uint32_t item) {
     const uint32_t image = item / s.groups, group = item % s.groups;
     if (image >= s.n) return nullptr;
-    return partial + ((size_t)(image * s.tiles + group / s.tile_groups) * s.tile_groups + group % s.tile_groups) * s.slabs;
+    return partial + ((size_t)(image * s.tiles + group / s.tile_groups * s.parts) * s.tile_groups + group % s.tile_groups) * s.slabs;
 }
 
 __global__ void __launch_bounds__(kThreads) k_combine_moments(const float2* __restrict__ partial, float2* __restrict__ moments, Shape s) {
@@ -684,11 +705,11 @@ __global__ void __launch_bounds__(kThreads) k_apply(const void* __restrict__ x, 
                                                     void* __restrict__ y, float2* __restrict__ moments, Shape s, Shape of_sums, Dropout d) {
     __shared__ float2 folded[kTileGroups];
     const Place p = place_of(s, blockIdx.x);
-    float2* of_tile = moments + (size_t)p.image * s.groups + p.tile * s.tile_groups;
+    float2* of_tile = moments + (size_t)p.image * s.groups + p.group;
     const float2* m = of_tile;
     if (partial) {
         fold_tile(partial, of_sums, p, folded, fold_moments);
-        if (p.slab == 0 && threadIdx.x < groups_of_tile(s, p.tile)) of_tile[threadIdx.x] = folded[threadIdx.x];
+        if (p.slab == 0 && p.part == 0 && threadIdx.x < p.groups) of_tile[threadIdx.x] = folded[threadIdx.x];
         m = folded;
     }
     const uint32_t row = thread_row(s, p, V);
@@ -731,7 +752,7 @@ __global__ void __launch_bounds__(kThreads) k_gradient_sums(const void* __restri
                                           }
                                       });
     }
-    const uint32_t groups = groups_of_tile(s, p.tile), first = p.tile * s.tile_groups, channels = groups * s.per_group;
+    const uint32_t groups = p.groups, first = p.group, channels = p.width;
     float2* mine = of_channels + ((size_t)p.image * s.slabs + p.slab) * s.channels + p.channel;
     float* totals = column_sums<2 * V>(total, s.columns, s.rows, lds);
     // a channel's two sums, and weighted in place
@@ -747,7 +768,7 @@ __global__ void __launch_bounds__(kThreads) k_gradient_sums(const void* __restri
     const uint32_t lanes = lanes_for(groups), lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
     float a = 0.0f, b = 0.0f;
     if (group < groups)
-        for (uint32_t i = group * s.per_group + lane; i < (group + 1) * s.per_group; i += lanes) {
+        for (uint32_t i = group * p.group_width + lane; i < (group + 1) * p.group_width; i += lanes) {
             const float* of_channel = totals + i / V * (2 * V) + i % V;
             a += of_channel[0];
             b += of_channel[V];
@@ -772,7 +793,7 @@ __global__ void __launch_bounds__(kThreads) k_input_gradient(const void* __restr
         return;
     }
     const Place p = place_of(s, blockIdx.x - parameter_blocks);
-    const float2* ab = means + (size_t)p.image * s.groups + p.tile * s.tile_groups;
+    const float2* ab = means + (size_t)p.image * s.groups + p.group;
     if (!means) {
         fold_tile(of_groups, of_sums, p, folded, fold_gradients);
         ab = folded;
@@ -830,7 +851,7 @@ inline Shape base_shape(const inpc_group_norm_config& cfg) {
 constexpr uint64_t kSingleBytes = 64 * 1024;
 
 // Groups of a tile of the split form with vectors of v elements: as many as fit, with boundaries on vectors' boundaries; 0 where
-// not even the fewest do.
+// not even the fewest do (nor do they then with shorter vectors, which fill a block with as many fewer channels).
 inline uint32_t tile_groups_of(const inpc_group_norm_config& cfg, int v) {
     const uint32_t per_group = cfg.channels / cfg.groups;
     uint32_t unit = 1;   // groups whose channels are whole vectors
@@ -839,9 +860,19 @@ inline uint32_t tile_groups_of(const inpc_group_norm_config& cfg, int v) {
     return (uint32_t)std::min<uint64_t>(cfg.groups, fit / unit * unit);
 }
 
+// Tiles of each group where it is too wide for one; v divides its channels.
+inline uint32_t parts_of(const inpc_group_norm_config& cfg, int v) { return div_up(cfg.channels / cfg.groups / (uint32_t)v, kThreads); }
+
+// Blocks of a launch: fewer than 2^32 threads, with room for the blocks that add up the parameters' gradients
+constexpr uint64_t kMostBlocks = 0xFFFFFFFFu / kThreads - INPC_GROUP_NORM_MAX_CHANNELS / kParameterColumns;
+
+// A group that is too wide for a block (4096 values of 16 bits, 512 single elements) is cut into parts, so that neither a whole image's
+// time nor its chains of additions are one block's: forward and backward of 200x200x515 fp16 in one group take 61 ms in the single form and
+// 0.21 ms in parts, of 64 images of 16x16x515 350 and 146 us. The single form stays where parts would take more blocks than a launch
+// has: such images have few pixels.
 inline bool runs_single(const inpc_group_norm_config& cfg, int v) {
     const uint64_t bytes = (uint64_t)cfg.n_pixels * (cfg.channels / cfg.groups) * element_bytes(cfg.dtype);
-    return bytes <= kSingleBytes || tile_groups_of(cfg, v) == 0;
+    return bytes <= kSingleBytes || (tile_groups_of(cfg, v) == 0 && (uint64_t)cfg.n_images * cfg.groups * parts_of(cfg, v) > kMostBlocks);
 }
 
 // Threads of a block of the single form: as many as the group has vectors, in whole waves.
@@ -862,8 +893,17 @@ inline uint64_t map_bytes(const inpc_group_norm_config& cfg) {
 inline Shape split_shape(const inpc_group_norm_config& cfg, int v, uint32_t blocks) {
     Shape s = base_shape(cfg);
     s.tile_groups = tile_groups_of(cfg, v);
-    s.tiles = div_up(s.groups, s.tile_groups);
-    s.columns = s.tile_groups * s.per_group / (uint32_t)v;
+    s.parts = 1;
+    if (s.tile_groups != 0) {
+        s.tiles = div_up(s.groups, s.tile_groups);
+        s.columns = s.tile_groups * s.per_group / (uint32_t)v;
+    } else {
+        s.tile_groups = 1;
+        s.parts = parts_of(cfg, v);
+        s.tiles = s.groups * s.parts;
+        s.columns = div_up(s.per_group / (uint32_t)v, s.parts);
+    }
+    s.tile_channels = s.columns * (uint32_t)v;
     s.rows = kThreads / s.columns;
     const uint64_t runs = (uint64_t)s.n * s.tiles, per_run = std::max<uint64_t>(1, blocks / runs);
     const uint64_t wanted = (s.pixels + per_run - 1) / per_run;
@@ -887,7 +927,12 @@ inline bool streams(const inpc_group_norm_config& cfg, int maps) {
     return map_bytes(cfg) * maps > kStreamedBytes;
 }
 
-inline bool folds(const Shape& s) { return (uint64_t)s.slabs * s.tile_groups <= kFoldedSums; }
+inline bool folds(const Shape& s) { return (uint64_t)s.slabs * s.parts * s.tile_groups <= kFoldedSums; }
+
+// Whether a call may run with vectors of v elements: a group in parts is whole vectors
+inline bool vector_fits(const inpc_group_norm_config& cfg, int v) {
+    return (tile_groups_of(cfg, v) != 0 ? cfg.channels : cfg.channels / cfg.groups) % (uint32_t)v == 0;
+}
 
 // What a call may need: [sums per (image, tile, group of a tile, slab)] [backward: sums per (image, slab, channel)] [means per
 // (image, group)], the second with one slab in the single form.
@@ -906,7 +951,7 @@ inline Workspace split_workspace(const Shape& s, bool backward) {
 inline size_t workspace_bytes(const inpc_group_norm_config& cfg, bool backward) {
     size_t most = backward && cfg.n_images > 1 ? (size_t)cfg.n_images * cfg.channels * sizeof(float2) : 0;
     for (int v = (int)(16 / element_bytes(cfg.dtype)); v >= 1; v /= 2)
-        if (cfg.channels % (uint32_t)v == 0 && !runs_single(cfg, v))
+        if (vector_fits(cfg, v) && !runs_single(cfg, v))
             most = std::max(most, split_workspace(sums_shape(cfg, v), backward).bytes);
     return most;
 }
@@ -1072,9 +1117,10 @@ inline int forward(const inpc_group_norm_config& cfg, const void* x, const void*
     const size_t bytes = element_bytes(cfg.dtype);
     const uint64_t divisible = cfg.channels | cfg.input_image_stride | cfg.input_pixel_stride;
     const uintptr_t pointers = (uintptr_t)x | (uintptr_t)y;
-    const int v = vector_width(bytes, divisible, pointers);
-    if (!runs_single(cfg, v)) return INPC_NORM_DISPATCH(forward_split, cfg.dtype, v, cfg, x, weight, bias, y, moments, ws, stream);
+    int v = vector_width(bytes, divisible, pointers);
     const int in_group = vector_width(bytes, divisible | cfg.channels / cfg.groups, pointers);
+    if (tile_groups_of(cfg, v) == 0) v = in_group;
+    if (!runs_single(cfg, v)) return INPC_NORM_DISPATCH(forward_split, cfg.dtype, v, cfg, x, weight, bias, y, moments, ws, stream);
     return INPC_NORM_DISPATCH(forward_single, cfg.dtype, in_group, cfg, x, weight, bias, y, moments, stream);
 }
 
@@ -1083,10 +1129,11 @@ inline int backward(const inpc_group_norm_config& cfg, const void* x, const void
     const size_t bytes = element_bytes(cfg.dtype);
     const uint64_t divisible = cfg.channels | cfg.input_image_stride | cfg.input_pixel_stride | cfg.grad_image_stride | cfg.grad_pixel_stride;
     const uintptr_t pointers = (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx;
-    const int v = vector_width(bytes, divisible, pointers);
+    int v = vector_width(bytes, divisible, pointers);
+    const int in_group = vector_width(bytes, divisible | cfg.channels / cfg.groups, pointers);
+    if (tile_groups_of(cfg, v) == 0) v = in_group;
     if (!runs_single(cfg, v))
         return INPC_NORM_DISPATCH(backward_split, cfg.dtype, v, cfg, x, dy, moments, weight, bias, dx, dweight, dbias, ws, stream);
-    const int in_group = vector_width(bytes, divisible | cfg.channels / cfg.groups, pointers);
     return INPC_NORM_DISPATCH(backward_single, cfg.dtype, in_group, cfg, x, dy, moments, weight, bias, dx, dweight, dbias, ws, stream);
 }
 

@@ -220,6 +220,31 @@ def test_group_norm_of_large_groups(gpu, shape):
     check(*make_case(*size, dtype, sum(size)), groups, act, p=p, seed=19)
 
 
+# groups too wide for a block: each is cut into parts
+WIDE_SHAPES = [
+    (2, 1030, 40, 11, 2, "bf16", "silu", 0.25),     # vectors of two would end inside a part: single elements, parts of 258 and 257
+    (1, 8008, 12, 9, 8, "fp16", "gelu", 0.0),       # 1001 channels to a group, two parts each
+    (3, 4104, 9, 7, 1, "fp16", "relu", 0.1),        # 513 vectors of eight
+    (1, 6148, 5, 5, 1, "fp32", "none", 0.5),        # four parts, the last one narrower
+    (2, 2052, 31, 20, 1, "fp32", "silu", 0.0),
+]
+
+
+@pytest.mark.parametrize("shape", WIDE_SHAPES, ids=str)
+def test_group_norm_of_wide_groups(gpu, shape):
+    *size, groups, dtype, act, p = shape
+    x, weight, bias, dy = make_case(*size, dtype, sum(size))
+    check(x, weight, bias, dy, groups, act, p=p, seed=19)
+    # from an odd channel of a wider map: single elements
+    check(x, weight, bias, dy, groups, act, p=p, seed=19, on_device=lambda t: to_device(torch.cat((t[:, :3], t, t[:, :2]), 1))[:, 3:-2])
+
+
+def test_group_norm_gradients_of_a_wide_group_with_many_pixels(gpu):
+    """Equal values, so that every addition of a long chain would round the same way."""
+    x, weight, bias, dy = make_case(1, 515, 200, 200, "fp16", 29)
+    check(x, weight, bias, torch.full_like(dy, 0.1), 1)
+
+
 def test_group_norm_some_gradients_of_large_groups(gpu):
     x, weight, bias, dy = make_case(2, 8, 100, 90, "fp32", 77)
     ref = R.GroupNorm(x, 2, weight, bias, 1e-5, "silu", None, dy)
@@ -748,6 +773,24 @@ def test_an_outlier_in_front_of_long_runs(gpu):
     for image in (0, 511):
         ref = R.GroupNorm(x[image:image + 1].cpu(), 32, None, None, 1e-5, "none")
         R.assert_within(y[image:image + 1], ref.y, ref.y_bound, "y")
+
+
+@pytest.mark.real_gpu
+def test_wide_groups_of_more_images_than_parts_have_blocks(gpu):
+    """65600 images of one pixel, 65535 channels each, in one group: a block for each, and more than 2^32 values in both directions."""
+    n, c = 65600, 65535
+    assert n * c > 2**32
+    gen = torch.Generator(device=gpu).manual_seed(4)
+    x, dy = (torch.empty(n, c, dtype=torch.float16, device=gpu).normal_(generator=gen).view(n, c, 1, 1) for _ in range(2))
+    x.requires_grad_(True)
+    y = group_norm(x, 1, activation="silu", dropout_p=0.25, seed=7)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for image in (0, 40000, n - 1):
+        keep = torch.from_numpy(R.kept(image * c, c, 0.25, 7, 0)).view(1, c, 1, 1).double() / 0.75
+        part = slice(image, image + 1)
+        ref = R.GroupNorm(x[part].detach().cpu(), 1, None, None, 1e-5, "silu", keep, dy[part].cpu())
+        R.assert_within(y[part], ref.y, ref.y_bound, "y")
+        R.assert_within(dx[part], ref.dx, ref.dx_bound, "dx")
 
 
 @pytest.mark.real_gpu

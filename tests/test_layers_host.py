@@ -116,6 +116,23 @@ def test_refused_pointers_and_workspaces():
     assert lib.inpc_dropout(None, None, 0, 0, 0.5, 1, None, 0, None) == 0
 
 
+def test_wide_groups_take_a_workspace_where_they_are_cut_into_parts():
+    lib = _lib.lib()
+
+    def sizes(**changes):
+        cfg = config(**changes)
+        return [lib.inpc_group_norm_workspace_bytes(C.byref(cfg), backward) for backward in (0, 1)]
+
+    wide = dict(channels=65535, groups=1, n_pixels=1, input_pixel_stride=65535, input_image_stride=65535, grad_pixel_stride=65535,
+                grad_image_stride=65535)
+    # 128 parts of 512 single elements at most, one slab: a pair of sums for each, of each channel, and of each image
+    assert sizes(**wide, n_images=1000) == [1000 * 128 * 8, 1000 * 128 * 8 + (1000 * 65535 * 8 + 255) // 256 * 256 + 1000 * 8]
+    # more blocks than a launch has: a block for each image
+    assert sizes(**wide, n_images=65600) == [0, 65600 * 65535 * 8]
+    # 64 KB: one block
+    assert sizes(**dict(wide, channels=32768), n_images=2) == [0, 2 * 32768 * 8]
+
+
 def test_operators_refuse_host_tensors():
     x = torch.randn(1, 4, 2, 2)
     with pytest.raises(RuntimeError, match="GPU"):

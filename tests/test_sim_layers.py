@@ -27,6 +27,10 @@ CASES = [
     ("test_group_norm_of_large_groups", dict(shape=(2, 24, 120, 95, 3, "fp16", "gelu", 0.25))),
     ("test_group_norm_of_large_groups", dict(shape=(1, 33, 200, 200, 33, "fp32", "silu", 0.1))),
     ("test_group_norm_of_large_groups", dict(shape=(1, 40, 120, 75, 5, "fp32", "relu", 0.0))),
+    *(("test_group_norm_of_wide_groups", dict(shape=shape))
+      for shape in ((2, 1030, 40, 11, 2, "bf16", "silu", 0.25), (1, 8008, 12, 9, 8, "fp16", "gelu", 0.0), (3, 4104, 9, 7, 1, "fp16", "relu", 0.1),
+                    (1, 6148, 5, 5, 1, "fp32", "none", 0.5))),
+    ("test_group_norm_gradients_of_a_wide_group_with_many_pixels", {}),
     ("test_group_norm_activation_and_dropout", dict(act="silu", p=0.35, dtype="bf16")),
     ("test_group_norm_layouts", dict(dtype="bf16")),
     ("test_group_norm_of_values_far_from_zero", {}),
@@ -96,7 +100,7 @@ def test_the_seed_of_a_call_without_dropout_is_not_read(sim):
 
 @pytest.mark.parametrize("order", ["reverse", "shuffle"])
 def test_results_do_not_depend_on_the_order_of_threads_and_blocks(order):
-    chosen = [_case_id(c) for c in CASES if "large_groups" in c[0] or c[0] in ("test_group_norm", "test_dropout_layouts")]
+    chosen = [_case_id(c) for c in CASES if "large_groups" in c[0] or "wide_groups" in c[0] or c[0] in ("test_group_norm", "test_dropout_layouts")]
     nodes = [f"{Path(__file__)}::test_on_the_simulator[{case}]" for case in chosen]
     done = subprocess.run([sys.executable, "-m", "pytest", *nodes, "-q", "-x", "-p", "no:cacheprovider"],
                           env=dict(os.environ, INPC_SIM_ORDER=order), capture_output=True, text=True, stdin=subprocess.DEVNULL,
