@@ -39,11 +39,15 @@ constexpr uint32_t kSumBlocks = 512;
 constexpr uint32_t kSmallSumBlocks = 256;
 constexpr uint64_t kSmallMap = 48ull << 20;
 // Where the sums of a tile of an image are at most this many, every applying block adds them up itself; beyond a launch in
-// between does. 65 MB, 8 groups (4000 sums): apply 27 us against 23 us + 4.4 us; 33 MB, 32 groups (8000 sums): 20 us against
+// between does: for 17 to 32 groups in one tile of one image of more than 48 MB, and for maps of gigabytes (kLongestRun). 65 MB, 8 groups (4000 sums): apply 27 us against 23 us + 4.4 us; 33 MB, 32 groups (8000 sums): 20 us against
 // 16 us + 4.5 us, and a launch less for the host; the same with 16000 sums: 26 us against 16 us + 4.5 us.
 constexpr uint32_t kFoldedSums = 8192;
 // Blocks of a launch that applies and does not add up. 65 MB: 22.7 us with 1024, 23.4 with 2048, 27.9 with 4096.
 constexpr uint32_t kApplyBlocks = 1024;
+// Vectors of a thread at most: a longer chain of fp32 additions costs digits (five images of 4100x4100x64 bf16 with 2575 each: the
+// parameters' gradients of equal values were off by 280 u). Larger maps, of more than 2 GB, take two, three, ... times the blocks: whole rounds of
+// them cost nothing (2.3 to 2.7 GB forward and backward 3.7 to 4.3 ms either way), a fourth more blocks cost a tenth.
+constexpr uint32_t kLongestRun = 512;
 constexpr uint32_t kTileGroups = 32;     // groups of a tile of channels at most: a block's threads share them out at once
 constexpr uint32_t kParameterColumns = 32;
 
@@ -905,7 +909,9 @@ inline Shape split_shape(const inpc_group_norm_config& cfg, int v, uint32_t bloc
     }
     s.tile_channels = s.columns * (uint32_t)v;
     s.rows = kThreads / s.columns;
-    const uint64_t runs = (uint64_t)s.n * s.tiles, per_run = std::max<uint64_t>(1, blocks / runs);
+    const uint64_t runs = (uint64_t)s.n * s.tiles, longest = (uint64_t)s.rows * kLongestRun;
+    uint64_t per_run = std::max<uint64_t>(1, blocks / runs);
+    per_run *= (s.pixels + per_run * longest - 1) / (per_run * longest);   // whole rounds of blocks
     const uint64_t wanted = (s.pixels + per_run - 1) / per_run;
     const uint32_t step = s.rows * kUnroll;
     s.slab_pixels = (uint32_t)((wanted + step - 1) / step * step);

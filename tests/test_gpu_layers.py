@@ -794,6 +794,66 @@ def test_wide_groups_of_more_images_than_parts_have_blocks(gpu):
 
 
 @pytest.mark.real_gpu
+def test_gradients_of_more_than_two_to_the_32_values(gpu):
+    """Five images of 4100x4100x64 bf16. A channel's gradients are sums over 84 million pixels: a thread's own run (512 at most), the
+    block's 64 rows, 2600 slabs by 16 threads and those: not 1000 roundings one after the other."""
+    roundings = 1000
+    n, c, h, w = 5, 64, 4100, 4100
+    x, dy = (torch.zeros((n, h, w, c), dtype=torch.bfloat16, device=gpu).permute(0, 3, 1, 2) for _ in range(2))
+    weight = torch.ones(c, device=gpu).requires_grad_(True)
+    bias = torch.zeros(c, device=gpu).requires_grad_(True)
+    # Equal values, 0.1 times the slope at 0.3, which fills the mantissa. Within a binade of its sum every addition of a chain of L is off
+    # by the same amount, half a step at most: 2/3 L u 2^k where the sum ends at 2^k + 2^k, so L u / 3, and 0.37 L u where it ends half-way
+    # to there. With runs of 512 and 163 slabs to a thread, and 16 u for the slope, the joins and the store: 266 u.
+    dy.fill_(0.1)
+    at = torch.full((c,), 0.3, device=gpu).requires_grad_(True)
+    (dbias,) = torch.autograd.grad(group_norm(x, 4, weight, at, activation="silu"), at, dy)
+    each = float(dy[0, 0, 0, 0]) * R.slope(at.detach().cpu().double(), "silu")
+    R.assert_within(dbias, n * h * w * each, 266 * R.U * n * h * w * each, "dbias of equal values")
+    # the last image alone: its values start behind 2^32
+    gen = torch.Generator(device=gpu).manual_seed(1)
+    dy.zero_()
+    x[-1].normal_(generator=gen)
+    dy[-1].normal_(generator=gen)
+    x.requires_grad_(True)
+    dx, dweight, dbias = torch.autograd.grad(group_norm(x, 4, weight, bias, activation="silu"), (x, weight, bias), dy)
+    assert not dx[:-1].any()
+    for group in (0, 3):
+        part = slice(16 * group, 16 * group + 16)
+        with torch.no_grad():
+            ref = R.GroupNorm(x[-1:, part], 1, None, None, 1e-5, "silu", None, dy[-1:, part])
+        more = roundings / (32 + 8 * 16 + 256 / 16)   # than the reference allows for
+        R.assert_within(dx[-1:, part], ref.dx, more * ref.dx_bound, "dx")
+        R.assert_within(dweight[part], ref.dweight, more * ref.dweight_bound, "dweight")
+        R.assert_within(dbias[part], ref.dbias, more * ref.dbias_bound, "dbias")
+        del ref
+
+
+@pytest.mark.real_gpu
+def test_slab_sums_of_two_images_and_tiles_in_a_launch_of_their_own(gpu):
+    """Two images of 4200x4200x64 fp16 in 64 groups, two tiles of 32 with 384 slabs each: more sums than every block adds up itself. Longest way
+    of a value: a run of 512, a block's 128 rows, 384 slabs by 64 lanes: not 1000 roundings."""
+    roundings, n, c, h, w = 1000, 2, 64, 4200, 4200
+    gen = torch.Generator(device=gpu).manual_seed(5)
+    x, dy = (torch.empty(n, h, w, c, dtype=torch.float16, device=gpu).normal_(generator=gen).permute(0, 3, 1, 2) for _ in range(2))
+    weight, bias = (torch.randn(c, generator=gen, device=gpu).requires_grad_(True) for _ in range(2))
+    x.requires_grad_(True)
+    with _lib.KernelTimer() as timer:
+        y = group_norm(x, 64, weight, bias, activation="silu")
+    assert [name for name, _ in timer.records] == ["group_norm_moments", "group_norm_combine_moments", "group_norm_apply"]
+    dx, dweight, dbias = torch.autograd.grad(y, (x, weight, bias), dy)
+    for channel in (0, 31, 32, 63):
+        part = slice(channel, channel + 1)
+        with torch.no_grad():
+            ref = R.GroupNorm(x[:, part], 1, weight[part], bias[part], 1e-5, "silu", None, dy[:, part])
+        more = roundings / (32 + 8 + 256)   # than the reference allows for
+        R.assert_within(y[:, part], ref.y, more * ref.y_bound, "y")
+        R.assert_within(dx[:, part], ref.dx, more * ref.dx_bound, "dx")
+        R.assert_within(dweight[part], ref.dweight, more * ref.dweight_bound, "dweight")
+        R.assert_within(dbias[part], ref.dbias, more * ref.dbias_bound, "dbias")
+
+
+@pytest.mark.real_gpu
 def test_a_map_beyond_the_caches(gpu):
     """A map of 102 MB in 20 groups: more slab sums than every block adds up itself, and results that are stored past the caches."""
     gen = torch.Generator(device=gpu).manual_seed(3)
