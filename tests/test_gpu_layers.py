@@ -735,6 +735,115 @@ def test_calls_on_two_streams_at_once(gpu):
             assert torch.equal(a, y) and torch.equal(b, dx)
 
 
+def large_step(n, c, h, w, groups, dtype, seed):
+    """A training step of a map whose groups are too large for a block each: its slab sums lie in a workspace in both directions.
+    Returns the input and step(seed of the mask), which gives the output and all gradients."""
+    x, weight, bias, dy = (to_device(t) for t in make_case(n, c, h, w, dtype, seed))
+    for t in (x, weight, bias):
+        t.requires_grad_(True)
+
+    def step(mask_seed):
+        y = group_norm(x, groups, weight, bias, activation="silu", dropout_p=0.2, seed=mask_seed, offset=7)
+        return (y, *torch.autograd.grad(y, (x, weight, bias), dy))
+
+    with _lib.KernelTimer() as timer:
+        group_norm(x.detach(), groups, weight, bias)
+    assert "group_norm_moments" in [name for name, _ in timer.records]
+    return x, step
+
+
+LARGE_STEPS = [(1, 16, 200, 150, 4, "fp16"), (2, 24, 120, 95, 3, "fp32"), (2, 1030, 40, 11, 2, "bf16")]   # the last in parts
+
+
+@pytest.mark.real_gpu
+@pytest.mark.parametrize("shape", LARGE_STEPS, ids=str)
+def test_captured_steps_of_large_groups(gpu, shape):
+    """Two graphs, replayed on two streams at once, with eager steps and new inputs between the replays."""
+    held = torch.tensor([100], dtype=torch.int64, device=gpu)
+    graphs, kept = [], []
+    for k in range(2):
+        x, step = large_step(*shape, 80 + k)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(held)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = [t.detach() for t in step(held)]
+        graphs.append(graph)
+        kept.append((x, step, captured))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for replay in range(4):
+        held.fill_(1000 + replay)
+        with torch.no_grad():
+            for x, _, _ in kept:
+                x.copy_(torch.randn_like(x))
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, step, captured in kept:
+            got = [t.clone() for t in captured]
+            eager = step(1000 + replay)
+            torch.cuda.synchronize()
+            for a, b in zip(got, eager):
+                assert torch.equal(a, b), replay
+
+
+@pytest.mark.real_gpu
+@pytest.mark.parametrize("shape", LARGE_STEPS, ids=str)
+def test_all_gradients_on_two_streams_at_once(gpu, shape):
+    steps = [large_step(*shape, 90 + k)[1] for k in range(2)]
+    want = [[t.detach().clone() for t in step(5)] for step in steps]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in steps], [[], []]
+    for _ in range(5):
+        for k, step in enumerate(steps):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(step(5))
+    torch.cuda.synchronize()
+    for results, expected in zip(got, want):
+        for result in results:
+            for a, b in zip(result, expected):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.real_gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_a_16_bit_map_beyond_the_caches(gpu, dtype):
+    """106 MB: results of both directions are stored past the caches."""
+    gen = torch.Generator(device=gpu).manual_seed(6)
+    x, dy = (torch.randn(1, 1300, 640, 64, generator=gen, device=gpu).to(DTYPES[dtype]).permute(0, 3, 1, 2) for _ in range(2))
+    weight, bias = (torch.randn(64, generator=gen, device=gpu) for _ in range(2))
+    leaves = [t.requires_grad_(True) for t in (x, weight, bias)]
+    y = group_norm(x, 8, weight, bias, activation="gelu")
+    grads = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        ref = R.GroupNorm(x, 8, weight, bias, 1e-5, "gelu", None, dy)
+        R.assert_within(y, ref.y, ref.y_bound, "y")
+        for got, name in zip(grads, ("dx", "dweight", "dbias")):
+            R.assert_within(got, getattr(ref, name), getattr(ref, name + "_bound"), name)
+
+
+@pytest.mark.real_gpu
+@pytest.mark.parametrize("pin_memory", [False, True])
+def test_saved_tensors_on_the_host(gpu, pin_memory):
+    x, weight, bias, dy = make_case(2, 16, 90, 101, "fp16", 33)
+    held = torch.tensor([12], device=gpu)
+    for map_on_device in (to_device, lambda t: to_device(torch.cat((t, t, t), 1))[:, 16:32]):
+        results = []
+        for on_host in (False, True):
+            leaves = [t.requires_grad_(True) for t in (map_on_device(x), to_device(weight), to_device(bias))]
+            with torch.autograd.graph.save_on_cpu(pin_memory) if on_host else torch.enable_grad():
+                y = dropout(group_norm(leaves[0], 4, *leaves[1:], activation="silu", dropout_p=0.2, seed=held), 0.1, held, offset=1)
+            results.append((y, *torch.autograd.grad(y, leaves, to_device(dy))))
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.real_gpu
 def test_more_than_two_to_the_32_values(gpu):
     # dropout: the block number passes 2^29, element numbers and byte offsets pass 2^32
