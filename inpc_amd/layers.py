@@ -19,31 +19,37 @@ _ACTIVATIONS = {"none": _lib.ACTIVATION_NONE, "relu": _lib.ACTIVATION_RELU, "sil
                 "gelu": _lib.ACTIVATION_GELU}
 
 
+_current_device, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _run(name: str, t: torch.Tensor, *args) -> None:
     """Calls the library with `args` and the current stream of the device that `t` lies on. The library launches on the
-    current device, so that is made the tensor's."""
-    index = t.get_device()
-    if index >= 0 and index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            _lib.check(getattr(_lib.lib(), name)(*args, _lib.current_stream()), name)
+    current device, so that is made the tensor's. Where it is already, device and stream are asked for without the layers that
+    torch.cuda puts around them (1 us of a small call's 10)."""
+    function, index = getattr(_lib.lib(), name), t.get_device()
+    if index < 0:
+        _lib.check(function(*args, _lib.current_stream()), name)
+    elif index == _current_device():
+        _lib.check(function(*args, _stream_of(index)), name)
     else:
-        _lib.check(getattr(_lib.lib(), name)(*args, _lib.current_stream()), name)
+        with torch.cuda.device(index):
+            _lib.check(function(*args, _stream_of(index)), name)
 
 
 def _address(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_tracing_state, _dispatch_mode, _PROXY = torch._C._get_tracing_state, torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
 
 
-def _require_plain_call(*tensors: torch.Tensor | None) -> None:
+def _require_plain_call(a: torch.Tensor, b: torch.Tensor | None = None, c: torch.Tensor | None = None, d: torch.Tensor | None = None) -> None:
     """Refuses what torch does around its own operators and would leave a kernel out of. The kernels compute no forward-mode
     derivatives, and what they write carries none; a recorded call would replay the allocation of the result alone."""
     if forward_ad._current_level >= 0:   # no dual tensors outside of a level: that alone is asked in most calls (0.07 us)
-        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (a, b, c, d)):
             raise RuntimeError("group_norm and dropout have no forward-mode derivative")
-    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+    if _tracing_state() is not None or _dispatch_mode(_PROXY) is not None:
         raise RuntimeError("group_norm and dropout cannot be recorded by torch.jit.trace or make_fx; capture a CUDA graph instead")
 
 
@@ -74,11 +80,14 @@ def _require_seed(seed: int | torch.Tensor | None, offset: int, device: torch.de
     return seed, None, offset
 
 
-def _require_unpacked(t: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype, grad: torch.Tensor) -> None:
-    """A hook on saved tensors gives back what it likes; the kernels go by the forward pass's sizes and types."""
-    if t is not None and (t.shape != shape or t.dtype != dtype or t.device != grad.device):
-        raise RuntimeError(f"a saved tensor of shape {tuple(shape)} and type {dtype} on {grad.device} was unpacked as {tuple(t.shape)}, "
-                           f"{t.dtype} on {t.device}")
+def _unpacked(t: torch.Tensor | None, count: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor | None:
+    """A saved vector as the kernels read it. A hook on saved tensors gives back what it likes, and the kernels go by the forward
+    pass's sizes and types."""
+    if t is None:
+        return None
+    if t.numel() != count or t.dtype != dtype or t.device != device:
+        raise RuntimeError(f"a saved vector, {count} of {dtype} on {device}, was unpacked as {t.numel()} of {t.dtype} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 # ---- dropout -------------------------------------------------------------------------------------------------------
@@ -98,9 +107,10 @@ def _dropout_call(x: torch.Tensor, p: float, seed: int, seed_tensor: torch.Tenso
 
 def _dropout_backward(ctx: Any, grad: torch.Tensor):
     _require_plain_call(grad)
-    p, seed, offset = ctx.random
-    (seed_tensor,) = ctx.saved_tensors or (None,)   # torch refuses one that has changed; a hook's copy keeps its value
-    _require_unpacked(seed_tensor, (1,), torch.int64, grad)
+    p, seed, seed_tensor, offset = ctx.random
+    if seed is None:
+        (seed_tensor,) = ctx.saved_tensors   # torch refuses one that has changed; a hook's copy keeps its value
+        seed, seed_tensor = 0, _unpacked(seed_tensor, 1, torch.int64, grad.device)
     return _dropout_call(grad.contiguous(memory_format=ctx.order), p, seed, seed_tensor, offset), None, None
 
 
@@ -111,10 +121,10 @@ _dropout_backward_once = once_differentiable(_dropout_backward)
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, order: torch.memory_format, random: tuple) -> torch.Tensor:
-        p, seed, seed_tensor, offset = random
-        ctx.order, ctx.random = order, (p, seed, offset)
-        if seed_tensor is not None:
-            ctx.save_for_backward(seed_tensor)   # torch watches over it
+        ctx.order, ctx.random = order, random
+        if random[2] is not None:
+            ctx.save_for_backward(random[2])   # torch watches over it
+            ctx.random = random[0], None, None, random[3]
         return _dropout_call(x, *random)
 
     @staticmethod
@@ -221,13 +231,16 @@ def _group_norm_backward(ctx: Any, grad: torch.Tensor):
     _require_plain_call(grad, x, weight, bias)
     cfg = _lib.GroupNormConfig.from_buffer_copy(ctx.cfg)   # two backward passes of one forward pass may run at once
     # Hooks on saved tensors may give back others than the forward pass's, which lie elsewhere and with other strides.
-    _require_unpacked(x, grad.shape, grad.dtype, grad)
-    _require_unpacked(weight, (cfg.channels,), ctx.param_dtype, grad)
-    _require_unpacked(bias, (cfg.channels,), ctx.param_dtype, grad)
-    _require_unpacked(moments, (2 * cfg.n_images * cfg.groups,), torch.float32, grad)
-    _require_unpacked(seed_tensor, (1,), torch.int64, grad)
-    x, cfg.input_image_stride, cfg.input_pixel_stride = _channels_last(x)
-    weight, bias, moments = (t if t is None else t.contiguous() for t in (weight, bias, moments))
+    device, (param_dtype, strides) = grad.device, ctx.saved_as
+    if x.shape != grad.shape or x.dtype != grad.dtype or x.device != device:
+        raise RuntimeError(f"the saved input, {tuple(grad.shape)} of {grad.dtype} on {device}, was unpacked as {tuple(x.shape)} of {x.dtype} "
+                           f"on {x.device}")
+    if x.stride() != strides:
+        x, cfg.input_image_stride, cfg.input_pixel_stride = _channels_last(x)
+    weight = _unpacked(weight, cfg.channels, param_dtype, device)
+    bias = _unpacked(bias, cfg.channels, param_dtype, device)
+    moments = _unpacked(moments, 2 * cfg.n_images * cfg.groups, torch.float32, device)
+    seed_tensor = _unpacked(seed_tensor, 1, torch.int64, device)
     cfg.seed_dev = _address(seed_tensor)
     grad, cfg.grad_image_stride, cfg.grad_pixel_stride = _channels_last(grad)
     need_x, need_weight, need_bias, _ = ctx.needs_input_grad
@@ -248,7 +261,7 @@ class _GroupNorm(torch.autograd.Function):
     def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, options: tuple) -> torch.Tensor:
         y, x, moments, ctx.cfg = _group_norm_call(x, weight, bias, *options)
         ctx.save_for_backward(x, weight, bias, moments, options[5])   # the last: a seed on the GPU, which torch watches over
-        ctx.param_dtype = next((t.dtype for t in (weight, bias) if t is not None), None)
+        ctx.saved_as = (weight.dtype if weight is not None else bias.dtype if bias is not None else None), x.stride()
         return y
 
     @staticmethod
