@@ -564,9 +564,9 @@ int inpc_cauchy_loss_backward(const float* grad, const float* input, const float
                               float* grad_input, uint32_t n, void* stream);
 
 /* =========================================================================================
- * Layers of the networks on either side of the rasterizer. The reference builds its own from torch's
- * (Modules/UNet.py:1-200, the network behind the image; Modules/AppearanceField.py:1-88, the one in front): these
- * calls have no counterpart among its kernels.
+ * Layers for networks on either side of the rasterizer, where the reference has a network of torch's layers behind the image
+ * (Modules/UNet.py:1-200) and a fused one of a third party in front (Modules/AppearanceField.py:1-88). These calls replace
+ * nothing of the reference's: neither operator is among its kernels.
  * ======================================================================================= */
 
 /* ---- element types and activations of the layers ------------------------------------------- */
@@ -598,7 +598,7 @@ typedef struct inpc_group_norm_config {
     uint64_t offset;
 } inpc_group_norm_config;
 
-/* The operators of the image network's blocks (Modules/UNet.py:1-200 takes its layers from torch):
+/* A block's normalisation and activation in a network that takes the rasterizer's images (the place of Modules/UNet.py:1-200):
  *   xhat = (x - mean) / sqrt(var + eps), mean and biased variance over the pixels of an image and the channels
  *   of a group; z = xhat * weight[c] + bias[c]; y = activation(z); with dropout_p > 0 then dropout of y, its
  *   elements numbered ((image * n_pixels) + pixel) * channels + c.
@@ -613,7 +613,7 @@ int inpc_group_norm_forward(const inpc_group_norm_config* cfg, const void* input
                             const void* bias, void* output, float* moments, void* workspace,
                             size_t workspace_bytes, void* stream);
 
-/* Gradients of the same (the layers of Modules/UNet.py:1-200): grad_input dense like the output, grad_weight and
+/* Gradients of the same (in a network in the place of Modules/UNet.py:1-200): grad_input dense like the output, grad_weight and
  * grad_bias (channels,) of param_dtype; any of the three may be NULL. `moments` is what the forward call wrote;
  * seed (or what seed_dev points to) and offset have to be those of the forward call: the mask is
  * computed again. A map without values (n_images or n_pixels 0) gives zeros in grad_weight and grad_bias; its forward call
@@ -623,13 +623,13 @@ int inpc_group_norm_backward(const inpc_group_norm_config* cfg, const void* grad
                              const float* moments, void* grad_input, void* grad_weight,
                              void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
 
-/* output[i] = 0 where u(i) < round(p * 2^32), else input[i] / (1 - p), computed in fp32 and rounded once (dropout of
- * hidden features, which a network like Modules/AppearanceField.py:1-88 takes from torch). The mask is stored nowhere:
+/* output[i] = 0 where u(i) < round(p * 2^32), else input[i] / (1 - p), computed in fp32 and rounded once: for the
+ * hidden features of a network that a user trains in the place of Modules/UNet.py:1-200 or Modules/AppearanceField.py:1-88. The mask is stored nowhere:
  * u(i) = h(0, i) * 2^16 + h(1, i), and h(d, i) is the 16-bit half i mod 8, low halves first, of the four words of
  * Philox4x32-10 with the seed as its key (low word first) and the counter (b mod 2^32, b div 2^32 + 2^31 d,
  * offset mod 2^32, offset div 2^32), b = i div 8. The backward pass is the same call on the gradient.
  * seed_dev, where not NULL, is read on the device in place of `seed`: a captured call then draws a new mask on
- * every replay whose seed was changed. output may be input. count < 2^40; p = 1 drops everything. */
+ * every replay whose seed was changed. p = 0 reads no seed. output may be input. count < 2^40; p = 1 drops everything. */
 int inpc_dropout(const void* input, void* output, uint64_t count, int dtype, double p,
                  uint64_t seed, const uint64_t* seed_dev, uint64_t offset, void* stream);
 

@@ -1,7 +1,7 @@
 // dropout.hpp — y = 0 where the mask drops the element, x / (1 - p) elsewhere; the backward pass is the same map on the
 // gradient, with the mask computed again (elements.hpp) instead of stored. x and y may be the same memory.
 //
-// What bounds it: memory. 8,388,352 x 64 bf16 values (1.07 GB) 340 us, 6.3 TB/s read and written; 65 MB of fp16 21 us (6.2 TB/s, in
+// What bounds it: memory. 8,388,352 x 64 bf16 values (1.07 GB) 340 us back to back, 6.3 TB/s read and written; 65 MB of fp16 21 us (6.2 TB/s, in
 // part from the memory-side cache). The generator's twenty products per eight values are hidden behind that; with a draw per
 // four values (32 bits each) they would take as long as the memory does for 16-bit types.
 #pragma once

@@ -13,8 +13,8 @@
 // taken from a value of the data, so that nothing cancels however far the values are from 0.
 //
 // What bounds it: memory. Forward reads x twice and writes y, backward reads x and dy twice and writes dx; up to some 200 MB
-// the second read comes from the 256 MB memory-side cache. 1240x824x32 fp16 (65 MB), SiLU: moments 15 us (4.4 TB/s), apply
-// 26 us (5.0 TB/s read and written), gradient sums 28 us (4.7 TB/s), input gradient 36 us (5.5 TB/s); without the activation the
+// the second read comes from the 256 MB memory-side cache. 1240x824x32 fp16 (65 MB), SiLU: moments 15 us (4.3 TB/s), apply
+// 27 us (4.8 TB/s read and written), gradient sums 29 us (4.5 TB/s), input gradient 37 us (5.3 TB/s); without the activation the
 // gradient sums take 26 us. A plain copy of that size reaches 5.9 TB/s from the cache and 4.9 TB/s from memory.
 #pragma once
 

@@ -2,8 +2,8 @@
 // the rasterizer's input:
 //   spherical contraction of the sample positions   (B/misc/src/misc_kernels.cu:49-66)
 //   raw density feature -> opacity and its gradient  (feature_to_opacity / TruncExp, utils.py:13-33)
-// and the layers of the networks there that the reference leaves to torch: group norm with an activation (groupnorm.hpp) and
-// dropout (dropout.hpp).
+// and layers for networks around these, which replace nothing of the reference's: group norm with an activation (groupnorm.hpp)
+// and dropout (dropout.hpp).
 #include <algorithm>
 
 #include "common.hpp"

@@ -1,7 +1,8 @@
-"""Layers of the networks on either side of the rasterizer: group norm with an activation over channels-last feature
-maps (with dropout behind it if asked for), and dropout from a counter-based generator. The reference builds its
-networks from torch's layers (Modules/UNet.py:1-200, Modules/AppearanceField.py:1-88); these two compute in fp32, run as
-hand-written kernels in both directions and keep neither normalised values nor masks for the backward pass.
+"""Layers for networks on either side of the rasterizer: group norm with an activation over channels-last feature
+maps (with dropout behind it if asked for), and dropout from a counter-based generator. Neither is among the reference's
+operators; they are for networks that a user trains in the places of Modules/UNet.py:1-200 and Modules/AppearanceField.py:1-88.
+Both compute in fp32, run as hand-written kernels in both directions and keep neither normalised values nor masks for the
+backward pass.
 """
 from __future__ import annotations
 
@@ -140,9 +141,10 @@ def dropout(input: torch.Tensor, p: float, seed: int | torch.Tensor | None, offs
     backward pass computes it again. Calls with different `seed` or `offset` draw independent masks, so use one seed for
     a training run and step the offset from layer to layer, and another seed for each iteration. `seed` is a whole
     number or a GPU tensor of one int64, which is read when the kernel runs (in a captured graph: on every
-    replay); torch refuses a backward pass if that tensor has been changed in between. The generator is
-    Philox4x32-10; include/inpc_hip.h (inpc_dropout) gives the numbering of its bits. With training=False or p = 0,
-    `input` itself is returned.
+    replay); torch refuses a backward pass if that tensor has been changed in between, and under hooks on saved tensors
+    (torch.utils.checkpoint, save_on_cpu) the saved value counts. The generator is Philox4x32-10; include/inpc_hip.h
+    (inpc_dropout) gives the numbering of its bits. With training=False or p = 0, `input` itself is returned. Second and
+    forward-mode derivatives are refused, and so is recording by torch.jit.trace or make_fx.
     """
     _require_values(input, "input")
     p = _require_probability(p, "p")
@@ -280,7 +282,7 @@ def group_norm(input: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     `bias` are (C,) tensors of one type, fp32 or the input's, so fp32 parameters serve 16-bit maps. Everything is
     computed in fp32 and rounded once, at the end of the whole chain. `dropout_p`, `seed`, `offset` and `training` are
     those of `dropout`, which gives the same mask for the same map. For the backward pass only the input and two
-    numbers per image and group are kept.
+    numbers per image and group are kept. What `dropout` refuses is refused here too.
     """
     _require_values(input, "input")
     if input.dim() != 4:

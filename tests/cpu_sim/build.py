@@ -11,8 +11,10 @@ operation against overflow, every conversion of a float to an integer against th
 GPU give different results); the first finding ends the process. The process has to start with the sanitizer's
 runtime preloaded:
 
-    LD_PRELOAD=$(gcc -print-file-name=libasan.so) ASAN_OPTIONS=detect_leaks=0 INPC_SIM_SANITIZE=1 \\
-        python -m pytest tests/test_sim_kernels.py -q
+    LD_PRELOAD="$(gcc -print-file-name=libasan.so) $(gcc -print-file-name=libstdc++.so)" ASAN_OPTIONS=detect_leaks=0 \\
+        INPC_SIM_SANITIZE=1 python -m pytest tests/test_sim_kernels.py -q
+
+(libstdc++ beside it, because torch throws in some of the tests and the runtime has to find what it stands in front of).
 """
 from __future__ import annotations
 
